@@ -317,6 +317,111 @@ int moba_step_layout(moba_step* step);
 int moba_forward_step(moba_step* step, void* stream);
 int moba_backward_step(moba_step* step, void* stream);
 
+/*
+ * Norm of queries and keys per head with the position rotation in the same
+ * pass (no counterpart in the reference). For every row x of D features:
+ * n = x (mean(x^2) + eps)^-1/2 w (n = x where the weight is NULL), then the
+ * first `rotary` features turned by the row's position: pairs (i, i +
+ * rotary / 2), or (2i, 2i + 1) where `interleaved`; the others stay. Computed
+ * in float32, rounded once.
+ * q [batch, seq, h_q, D], k [batch, seq, h_kv, D] by strides (batch, token,
+ * head of q, then of k; elements, multiples of 16 bytes, features next to
+ * each other); q_out, k_out contiguous. cos / sin [table_len, rotary / 2]
+ * float32. positions [batch * seq] int32, or NULL: 0, 1, .. in every row; a
+ * position outside the table gives NaN rows. Weights [D] of weight_dtype
+ * (float32 or the input dtype), or NULL. head_dim a power of two from 32 to
+ * 1024, rotary a multiple of 16. Rows on 16-byte boundaries.
+ * The backward takes the outputs' gradients (contiguous) and writes dq, dk
+ * (contiguous) and, for weights that are not NULL, their gradients, summed
+ * in a fixed order. Its workspace: moba_norm_rotate_bwd_workspace_size().
+ */
+int moba_norm_rotate(const void* q, const void* k, void* q_out, void* k_out,
+                     const float* cos_table, const float* sin_table, const int32_t* positions,
+                     const void* q_weight, const void* k_weight, int64_t batch, int64_t seq_len,
+                     int64_t h_q, int64_t h_kv, int64_t head_dim, const int64_t* strides,
+                     int64_t rotary, int64_t table_len, int interleaved, double eps, int dtype,
+                     int weight_dtype, void* stream);
+size_t moba_norm_rotate_bwd_workspace_size(int64_t head_dim);
+int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                         void* dq, void* dk, void* dq_weight, void* dk_weight,
+                         const float* cos_table, const float* sin_table,
+                         const int32_t* positions, const void* q_weight, const void* k_weight,
+                         int64_t batch, int64_t seq_len, int64_t h_q, int64_t h_kv,
+                         int64_t head_dim, const int64_t* strides, int64_t rotary,
+                         int64_t table_len, int interleaved, double eps, int dtype,
+                         int weight_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * New tokens of cached sequences (no counterpart in the reference). A page
+ * holds one MoBA block: k, v [n_pages, h_kv, block_size, D], kbar [n_pages,
+ * h_kv, D] (the blocks' representatives, written when a block becomes full).
+ * Row s of block_table [seqs, table_width] int32 lists the pages of sequence
+ * s in order; an entry outside [0, n_pages) is no page: tokens appended there
+ * are dropped, and attention sees no keys there. seq_lens[s] counts the
+ * sequence's tokens with its new ones, which are its last. cu_seqlens [seqs +
+ * 1] int32 packs the new tokens along the token axis (a sequence may have
+ * none); NULL: `even` tokens each. Rows of the token axis that belong to no
+ * sequence are neither read nor written, and sequences whose numbers make no
+ * sense (cu_seqlens outside the token axis or falling, seq_lens below the new
+ * tokens) have no new tokens. All of this is read on the device.
+ * Pages of one call's sequences that are appended to must be distinct; pages
+ * that are only read may be shared.
+ * head_dim 64, 128 or 256; block_size up to 1024; everything on 16-byte
+ * boundaries.
+ */
+typedef struct moba_paged {
+  int64_t tokens, seqs, h_q, h_kv, head_dim, block_size, table_width, n_pages, dtype, even;
+  int64_t slots, take, always_current; /* attention: as moba_gate */
+  int64_t workspace_bytes;             /* attention: set by moba_paged_layout */
+  const void* q;                       /* [tokens, h_q, D] */
+  void *k, *v, *kbar;
+  const int32_t *block_table, *seq_lens, *cu_seqlens;
+  int32_t* block_idx; /* attention: [tokens, h_q, slots] */
+  void* out;          /* attention: [tokens, h_q, D] */
+  float* lse;         /* attention: [h_q, tokens] in log2 units, or NULL */
+  void* workspace;
+} moba_paged;
+
+/*
+ * The new tokens' keys (normed and rotated as by moba_norm_rotate, at their
+ * positions in their sequences) and values into their pages, their queries to
+ * q_out [tokens, h_q, D], and the representatives of the blocks that became
+ * full, rounded as moba_pool rounds. strides: token, head of q, of k_new, of
+ * v_new. Tables, weights: as moba_norm_rotate (rotary 0: no rotation).
+ */
+int moba_append_tokens(const moba_paged* call, const void* k_new, const void* v_new,
+                       const int64_t* strides, void* q_out, const float* cos_table,
+                       const float* sin_table, const void* q_weight, const void* k_weight,
+                       int64_t rotary, int64_t table_len, int interleaved, double eps,
+                       int weight_dtype, void* stream);
+
+/*
+ * MoBA attention of the new tokens over the cache that holds them already.
+ * moba_paged_gate writes block_idx (moba_gate's rules: own block, `take` best
+ * strictly past blocks, ids ascending, -1 padded; all -1 for rows of no
+ * sequence), moba_paged_attend attends
+ * over the blocks of block_idx (keys behind a token's own position stay
+ * hidden; no visible key: out 0, lse -inf), moba_paged_attention does both.
+ * moba_paged_layout sets workspace_bytes from the first group of fields.
+ * take <= MOBA_PAGED_MAX_TAKE.
+ */
+#define MOBA_PAGED_MAX_TAKE 32
+int moba_paged_layout(moba_paged* call);
+int moba_paged_gate(const moba_paged* call, void* stream);
+int moba_paged_attend(const moba_paged* call, void* stream);
+int moba_paged_attention(const moba_paged* call, void* stream);
+
+/*
+ * Pages src[i] copied to dst[i], i < n, in all `layers` of k, v [layers,
+ * n_pages, h_kv, block_size, D] and kbar [layers, n_pages, h_kv, D]. The
+ * lists are on the host where `on_host` (read before the call returns), else
+ * on the device. Destinations must be distinct and no page both source and
+ * destination; pairs outside [0, n_pages) are skipped.
+ */
+int moba_copy_pages(void* k, void* v, void* kbar, const int32_t* src, const int32_t* dst,
+                    int64_t n, int on_host, int64_t layers, int64_t n_pages, int64_t h_kv,
+                    int64_t block_size, int64_t head_dim, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,80 @@
+// Sequences whose keys and values lie in the pages of a cache: addressing
+// shared by the kernels that write and read them.
+//
+// A page holds one MoBA block of every kv head: K and V [pages, h_kv, block,
+// D], so that a block of a head is one contiguous run, and the blocks'
+// representatives kbar [pages, h_kv, D]. Row s of the block table lists the
+// pages of sequence s in order; seq_lens[s] counts its tokens with the new
+// ones, which are its last. The new tokens of all sequences are packed along
+// one token axis by cu_seqlens (null: the same number for every sequence).
+#pragma once
+
+#include "common.h"
+
+namespace moba {
+
+struct Paged {
+  const int32_t* table;     // [seqs, width]
+  const int32_t* seq_lens;  // [seqs]
+  const int32_t* cu;        // [seqs + 1], or null
+  int32_t seqs, width, pages;
+  int32_t tokens;           // rows of the token axis
+  int32_t even;             // new tokens per sequence where cu is null
+  int32_t block;
+};
+
+// New tokens [first, first + n) of sequence s, at positions len - n, ..; n is
+// 0 where the values make no sense, so no caller's buffer leads a kernel out
+// of the token axis.
+struct NewTokens {
+  int32_t first, n, len;
+};
+
+__device__ inline NewTokens new_tokens(const Paged& p, int32_t s) {
+  NewTokens r;
+  r.first = p.cu ? p.cu[s] : s * p.even;
+  const int32_t end = p.cu ? p.cu[s + 1] : r.first + p.even;
+  r.len = p.seq_lens[s];
+  const bool ok = r.first >= 0 && end > r.first && end <= p.tokens && r.len >= end - r.first;
+  r.n = ok ? end - r.first : 0;
+  return r;
+}
+
+// Sequence and position of token `tok`, the same in all lanes of the wave;
+// position -1 where the token belongs to no sequence (rows behind the last
+// one, inconsistent lengths). Every lane compares one bound of 64, so up to
+// 64 sequences take one round of loads.
+struct TokenAt {
+  int32_t seq, pos;
+};
+
+__device__ inline TokenAt locate(const Paged& p, int32_t tok) {
+  int32_t s = 0;
+  if (p.cu) {
+    const int lane = threadIdx.x & 63;
+    for (int32_t base = 0; base < p.seqs; base += 64) {
+      const int32_t i = base + lane;
+      s += __popcll(__ballot(i < p.seqs && p.cu[i < p.seqs ? i + 1 : p.seqs] <= tok));
+    }
+  } else {
+    s = tok / p.even;
+  }
+  TokenAt t{s, -1};
+  if (s >= p.seqs) return t;
+  const NewTokens r = new_tokens(p, s);
+  const int32_t i = tok - r.first;
+  if (i >= 0 && i < r.n) t.pos = r.len - r.n + i;
+  return t;
+}
+
+// Page of block `blk` of sequence s, or -1 where the table has none.
+__device__ inline int32_t page_of(const Paged& p, int32_t s, int32_t blk) {
+  if (blk >= p.width) return -1;
+  const int32_t id = p.table[static_cast<int64_t>(s) * p.width + blk];
+  return id >= 0 && id < p.pages ? id : -1;
+}
+
+// Checks a call's shape and fills `p` (paged_attn.hip).
+int paged_of(const moba_paged* c, Paged* p);
+
+}  // namespace moba

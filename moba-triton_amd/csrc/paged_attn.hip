@@ -1,0 +1,522 @@
+// MoBA attention of new tokens over a paged cache.
+//
+// Gate: score(j) = T(float32(q . kbar_j)) for the strictly past blocks j < own
+// = position / block, the product exact (float64); the `take` best by (score
+// desc, block id asc), ids ascending, the own block last, -1 padding: the
+// rules of gate.hip. A block without a page (a table entry outside the cache)
+// never ranks. Attention: softmax(q . k / sqrt D) v over the chosen blocks'
+// keys up to the token's own position.
+#include "paged.h"
+#include "rotary.h"
+
+namespace moba {
+
+namespace {
+
+struct GateArgs {
+  Paged p;
+  const void* q;      // [tokens, h_q, D]
+  const void* kbar;   // [pages, h_kv, D]
+  uint32_t* keys;     // [slice tokens, h_q, width]
+  int32_t* block_idx; // [tokens, h_q, slots]
+  int32_t tok0, slice;  // tokens [tok0, tok0 + slice) of this launch
+  int h_q, h_kv, slots, take, current;
+};
+
+// A rounded score as an integer in the order of the scores, 0 for what never
+// ranks (-inf, NaN).
+__device__ inline uint32_t score_key(float rounded) {
+  const uint32_t u = f2u(rounded + 0.f);
+  const uint32_t o = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return o > 0x007fffffu && o <= 0xff800000u ? o : 0u;
+}
+
+// Scores of one token's query heads of one kv head against a run of its past
+// blocks: a block's representative belongs to D / 16 lanes, which hold it in
+// float64 for the heads of the group.
+constexpr int kScoreThreads = 256;
+constexpr int kScoreRows = 4;  // blocks per lane group
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kScoreThreads) score_kernel(GateArgs a) {
+  constexpr int D = 16 * LPR;
+  constexpr int G = kScoreThreads / LPR;
+  const int32_t local = blockIdx.x / a.h_kv;
+  const int hk = blockIdx.x % a.h_kv;
+  const TokenAt at = locate(a.p, a.tok0 + local);
+  if (at.pos < 0) return;
+  const int32_t own = at.pos / a.p.block;
+  const int32_t past = own < a.p.width ? own : a.p.width;
+  const int32_t j0 = blockIdx.y * (G * kScoreRows);
+  if (j0 >= past) return;
+  const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
+  const RotLane rl = rot_lane(lane, 0, 0);
+  const int group = a.h_q / a.h_kv;
+  const T* q = static_cast<const T*>(a.q) +
+               (static_cast<int64_t>(a.tok0 + local) * a.h_q + hk * group) * D;
+  for (int i = 0; i < kScoreRows; ++i) {
+    const int32_t j = j0 + i * G + g;
+    if (j >= past) break;
+    const int32_t page = page_of(a.p, at.seq, j);
+    double kd[16];
+    {
+      RawRow<T> raw;
+      raw.load(static_cast<const T*>(a.kbar) +
+                   (static_cast<int64_t>(page < 0 ? 0 : page) * a.h_kv + hk) * D, rl);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) kd[e] = static_cast<double>(raw.element(e));
+    }
+    for (int h = 0; h < group; ++h) {
+      RawRow<T> raw;
+      raw.load(q + h * D, rl);
+      double t = 0.0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t = fma(static_cast<double>(raw.element(e)), kd[e], t);
+#pragma unroll
+      for (int off = 1; off < LPR; off <<= 1) t += __shfl_xor(t, off);
+      if (lane == 0)
+        a.keys[(static_cast<int64_t>(local) * a.h_q + hk * group + h) * a.p.width + j] =
+            page < 0 ? 0u : score_key(Elem<T>::round(static_cast<float>(t)));
+    }
+  }
+}
+
+// The `take` best of a query's scores: one wave per (token, query head). Each
+// lane keeps the best TM of every 64th block, the lanes' lists meet in six
+// exchanges, each the best TM of two sorted lists.
+template <int TM>
+__global__ void __launch_bounds__(256) select_kernel(GateArgs a) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= static_cast<int64_t>(a.slice) * a.h_q) return;
+  const int lane = threadIdx.x & 63;
+  const TokenAt at = locate(a.p, a.tok0 + static_cast<int32_t>(row / a.h_q));
+  int32_t* out = a.block_idx + (static_cast<int64_t>(a.tok0) * a.h_q + row) * a.slots;
+  if (at.pos < 0) {
+    for (int i = lane; i < a.slots; i += 64) out[i] = -1;
+    return;
+  }
+  const int32_t own = at.pos / a.p.block;
+  const int32_t past = own < a.p.width ? own : a.p.width;
+  const uint32_t* keys = a.keys + row * a.p.width;
+  // (score, id) in one word, larger first: equal scores go to the lower id.
+  uint64_t best[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) best[i] = 0;
+  for (int32_t j = lane; j < past; j += 64) {
+    const uint32_t key = keys[j];
+    uint64_t x = key ? (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(j)) : 0;
+    if (x > best[TM - 1]) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const bool up = x > best[i];
+        const uint64_t t = up ? best[i] : x;
+        best[i] = up ? x : best[i];
+        x = t;
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    uint64_t other[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) other[i] = __shfl_xor(best[i], off);
+    // The larger of entry i and the other list's entry TM - 1 - i: the best
+    // TM of both, in an order that log2 TM exchange stages sort.
+#pragma unroll
+    for (int i = 0; i < TM; ++i) best[i] = best[i] > other[TM - 1 - i] ? best[i] : other[TM - 1 - i];
+#pragma unroll
+    for (int st = TM / 2; st > 0; st >>= 1)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        if ((i & st) == 0) {
+          const uint64_t x = best[i], y = best[i + st];
+          best[i] = x > y ? x : y;
+          best[i + st] = x > y ? y : x;
+        }
+  }
+  // Lane i takes entry i, and its place among the chosen ids.
+  uint32_t id = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+    if (i == lane && i < a.take && best[i]) id = 0xffffffffu - static_cast<uint32_t>(best[i]);
+  const uint64_t live = __ballot(id != 0xffffffffu);
+  int place = 0;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const uint32_t other = __shfl(id, i);
+    place += other < id ? 1 : 0;
+  }
+  int n = __popcll(live);
+  if (id != 0xffffffffu) out[place] = static_cast<int32_t>(id);
+  const bool cur = a.current && page_of(a.p, at.seq, own) >= 0;
+  if (cur && lane == 0) out[n] = own;
+  n += cur;
+  for (int i = n + lane; i < a.slots; i += 64) out[i] = -1;
+}
+
+struct RowArgs {
+  Paged p;
+  const void* q;             // [tokens, h_q, D]
+  const void* k;             // pages
+  const void* v;
+  const int32_t* block_idx;  // [tokens, h_q, slots]
+  void* out;                 // [tokens, h_q, D]
+  float* lse;                // [h_q, tokens] log2 units, or null
+  float* part_ml;            // [rows, splits, 2]
+  float* part_o;             // [rows, splits, D]
+  int h_q, h_kv, slots, splits;
+  float scale_log2;
+};
+
+constexpr int kRowWaves = 4;
+
+// One query head of one token per workgroup (and split): its chosen blocks in
+// runs of 64 / LPR * U keys, one run after another per wave. D / F lanes share
+// a key, F features each; every lane group keeps its own running maximum and
+// sum, and they meet at the end. All in float32.
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kRowWaves) attend_rows_kernel(RowArgs a) {
+  constexpr int F = 16 / static_cast<int>(sizeof(T));
+  constexpr int LPR = D / F;
+  constexpr int RPW = 64 / LPR;  // keys per load instruction
+  constexpr int U = 8;
+  constexpr int KEYS = RPW * U;
+  __shared__ float s_o[kRowWaves][D];
+  __shared__ float s_m[kRowWaves], s_l[kRowWaves];
+  const int64_t row = blockIdx.x;
+  const int32_t tok = static_cast<int32_t>(row / a.h_q);
+  const int h = static_cast<int>(row % a.h_q);
+  const int hk = h / (a.h_q / a.h_kv);
+  const TokenAt at = locate(a.p, tok);
+  if (at.pos < 0) return;  // its rows stay as they were
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = lane % LPR, g = lane / LPR;
+  const int bs = a.p.block;
+  float q[F];
+  {
+    const T* qp = static_cast<const T*>(a.q) + row * D + c * F;
+#pragma unroll
+    for (int e = 0; e < F; ++e) q[e] = Elem<T>::load(qp, e) * a.scale_log2;
+  }
+  float m = -INFINITY, l = 0.f, o[F];
+#pragma unroll
+  for (int e = 0; e < F; ++e) o[e] = 0.f;
+  const int per_block = (bs + KEYS - 1) / KEYS;
+  const int units = a.slots * per_block;
+  for (int u = blockIdx.y * kRowWaves + wave; u < units; u += a.splits * kRowWaves) {
+    const int32_t blk = a.block_idx[row * a.slots + u / per_block];
+    if (blk < 0) continue;
+    const int32_t page = page_of(a.p, at.seq, blk);
+    if (page < 0) continue;
+    const int64_t seen64 = static_cast<int64_t>(at.pos) - static_cast<int64_t>(blk) * bs + 1;
+    const int seen = seen64 < bs ? static_cast<int>(seen64) : bs;  // visible keys of the block
+    const int k0 = (u % per_block) * KEYS;
+    if (k0 >= seen) continue;
+    const int64_t base = (static_cast<int64_t>(page) * a.h_kv + hk) * bs * D + c * F;
+    const T* kp = static_cast<const T*>(a.k) + base;
+    const T* vp = static_cast<const T*>(a.v) + base;
+    rot_u32x4 kr[U], vr[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = k0 + i * RPW + g;
+      kr[i] = *reinterpret_cast<const rot_u32x4*>(kp + (r < seen ? r : seen - 1) * D);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = k0 + i * RPW + g;
+      vr[i] = *reinterpret_cast<const rot_u32x4*>(vp + (r < seen ? r : seen - 1) * D);
+      if (r >= seen) vr[i] = rot_u32x4{0, 0, 0, 0};  // hidden values add nothing, whatever they are
+    }
+    float s[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float t = 0.f;
+      const T* ke = reinterpret_cast<const T*>(&kr[i]);
+#pragma unroll
+      for (int e = 0; e < F; ++e) t = fmaf(q[e], Elem<T>::load(ke, e), t);
+      t = row_sum<LPR>(t);
+      s[i] = k0 + i * RPW + g < seen ? t : -INFINITY;
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < U; ++i) top = fmaxf(top, s[i]);
+    const float z = top > -INFINITY ? top : 0.f;
+    const float old = __builtin_amdgcn_exp2f(m - z);
+    l *= old;
+#pragma unroll
+    for (int e = 0; e < F; ++e) o[e] *= old;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float p = __builtin_amdgcn_exp2f(s[i] - z);
+      l += p;
+      const T* ve = reinterpret_cast<const T*>(&vr[i]);
+#pragma unroll
+      for (int e = 0; e < F; ++e) o[e] = fmaf(p, Elem<T>::load(ve, e), o[e]);
+    }
+    m = top;
+  }
+  // Lane groups, then waves.
+#pragma unroll
+  for (int off = LPR; off < 64; off <<= 1) {
+    const float om = __shfl_xor(m, off), ol = __shfl_xor(l, off);
+    const float top = fmaxf(m, om), z = top > -INFINITY ? top : 0.f;
+    const float wa = __builtin_amdgcn_exp2f(m - z), wb = __builtin_amdgcn_exp2f(om - z);
+    l = l * wa + ol * wb;
+#pragma unroll
+    for (int e = 0; e < F; ++e) o[e] = o[e] * wa + __shfl_xor(o[e], off) * wb;
+    m = top;
+  }
+  if (g == 0) {
+#pragma unroll
+    for (int e = 0; e < F; ++e) s_o[wave][c * F + e] = o[e];
+    if (c == 0) {
+      s_m[wave] = m;
+      s_l[wave] = l;
+    }
+  }
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, s_m[w]);
+  const float z = top > -INFINITY ? top : 0.f;
+  float total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) total += s_l[w] * __builtin_amdgcn_exp2f(s_m[w] - z);
+  for (int d = threadIdx.x; d < D; d += 64 * kRowWaves) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) x += s_o[w][d] * __builtin_amdgcn_exp2f(s_m[w] - z);
+    if (a.splits == 1)
+      Elem<T>::store(static_cast<T*>(a.out) + row * D, d, total > 0.f ? x / total : (total == 0.f ? 0.f : x + total));
+    else
+      a.part_o[(row * a.splits + blockIdx.y) * D + d] = x;
+  }
+  if (threadIdx.x == 0) {
+    if (a.splits > 1) {
+      a.part_ml[(row * a.splits + blockIdx.y) * 2] = top;
+      a.part_ml[(row * a.splits + blockIdx.y) * 2 + 1] = total;
+    } else if (a.lse) {
+      a.lse[h * static_cast<int64_t>(a.p.tokens) + tok] = total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
+    }
+  }
+}
+
+// Splits of a row merged: one wave per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(64) merge_rows_kernel(RowArgs a) {
+  const int64_t row = blockIdx.x;
+  const int32_t tok = static_cast<int32_t>(row / a.h_q);
+  if (locate(a.p, tok).pos < 0) return;
+  const float* ml = a.part_ml + row * a.splits * 2;
+  const float* po = a.part_o + row * a.splits * D;
+  float top = -INFINITY;
+  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, ml[2 * i]);
+  const float z = top > -INFINITY ? top : 0.f;
+  float total = 0.f, o[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+  for (int i = 0; i < a.splits; ++i) {
+    const float w = __builtin_amdgcn_exp2f(ml[2 * i] - z);
+    total += ml[2 * i + 1] * w;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] += po[i * D + 64 * e + threadIdx.x] * w;
+  }
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e)
+    Elem<T>::store(static_cast<T*>(a.out) + row * D, 64 * e + threadIdx.x,
+                   total > 0.f ? o[e] / total : (total == 0.f ? 0.f : o[e] + total));
+  if (a.lse && threadIdx.x == 0)
+    a.lse[(row % a.h_q) * static_cast<int64_t>(a.p.tokens) + tok] = total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
+}
+
+// How a call is cut up, and its workspace.
+struct PagedPlan {
+  int64_t slice;   // tokens per gate launch
+  int64_t splits;  // parts of a query's chosen blocks
+  size_t keys, ml, o, total;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Keys per run of attend_rows_kernel.
+int64_t run_keys(int64_t D, int dtype) { return 64 * 8 / (D / (dtype == MOBA_FP32 ? 4 : 8)); }
+
+PagedPlan plan_of(const moba_paged& c) {
+  PagedPlan pl;
+  const int64_t per_token = c.h_q * c.table_width;
+  pl.slice = (int64_t(1) << 24) / per_token;
+  pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
+  const int64_t rows = c.tokens * c.h_q;
+  const int64_t units = c.slots * cdiv(c.block_size, run_keys(c.head_dim, static_cast<int>(c.dtype)));
+  int64_t splits = cdiv(2048, rows * kRowWaves);
+  const int64_t most = cdiv(units, kRowWaves);
+  pl.splits = splits < most ? splits : most;
+  pl.keys = align256(sizeof(uint32_t) * static_cast<size_t>(pl.slice * per_token));
+  const size_t parts = pl.splits > 1 ? static_cast<size_t>(rows * pl.splits) : 0;
+  pl.ml = align256(sizeof(float) * 2 * parts);
+  pl.o = align256(sizeof(float) * c.head_dim * parts);
+  pl.total = pl.keys + pl.ml + pl.o;
+  return pl;
+}
+
+int check_attention(const moba_paged* c, Paged* p) {
+  const int st = paged_of(c, p);
+  if (st) return st;
+  if (c->slots <= 0 || c->take < 0 || c->take + (c->always_current ? 1 : 0) > c->slots)
+    return fail(MOBA_ERR_INVALID, "slots must hold the selected blocks");
+  if (c->take > MOBA_PAGED_MAX_TAKE)
+    return fail(MOBA_ERR_UNSUPPORTED, "more than " + std::to_string(MOBA_PAGED_MAX_TAKE) +
+                                          " past blocks per query");
+  if (c->tokens * c->h_q > (int64_t(1) << 31) - 1)
+    return fail(MOBA_ERR_UNSUPPORTED, "more than 2^31 - 1 query rows");
+  return MOBA_OK;
+}
+
+int check_workspace(const moba_paged* c, size_t need) {
+  if (!c->workspace || static_cast<size_t>(c->workspace_bytes) < need)
+    return fail(MOBA_ERR_WORKSPACE, "paged attention workspace too small");
+  return MOBA_OK;
+}
+
+bool aligned(const void* p) { return p && on_16_bytes(p); }
+
+}  // namespace
+
+int paged_of(const moba_paged* c, Paged* p) {
+  if (!c) return fail(MOBA_ERR_INVALID, "null pointer");
+  constexpr int64_t kMax = (int64_t(1) << 31) - 1;
+  for (int64_t n : {c->tokens, c->seqs, c->h_q, c->h_kv, c->head_dim, c->block_size,
+                    c->table_width, c->n_pages}) {
+    if (n <= 0) return fail(MOBA_ERR_INVALID, "non-positive shape argument");
+    if (n > kMax) return fail(MOBA_ERR_UNSUPPORTED, "a size exceeds 2^31 - 1");
+  }
+  if (c->h_q % c->h_kv)
+    return fail(MOBA_ERR_INVALID, "query heads " + std::to_string(c->h_q) +
+                                      " not divisible by kv heads " + std::to_string(c->h_kv));
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(MOBA_ERR_UNSUPPORTED, "paged caches take head_dim 64, 128 or 256");
+  if (c->block_size > 1024) return fail(MOBA_ERR_UNSUPPORTED, "block_size above 1024");
+  if (c->dtype < 0 || c->dtype > MOBA_FP32)
+    return fail(MOBA_ERR_UNSUPPORTED, "unknown dtype code");
+  *p = Paged{c->block_table, c->seq_lens, c->cu_seqlens, static_cast<int32_t>(c->seqs),
+             static_cast<int32_t>(c->table_width), static_cast<int32_t>(c->n_pages),
+             static_cast<int32_t>(c->tokens), static_cast<int32_t>(c->even),
+             static_cast<int32_t>(c->block_size)};
+  if (!p->table || !p->seq_lens) return fail(MOBA_ERR_INVALID, "null pointer");
+  if (!p->cu && (c->even <= 0 || c->even * c->seqs != c->tokens))
+    return fail(MOBA_ERR_INVALID,
+                "without cu_seqlens every sequence has the same number of new tokens");
+  if (c->table_width * c->block_size > kMax)
+    return fail(MOBA_ERR_UNSUPPORTED, "a sequence of the block table exceeds 2^31 - 1 tokens");
+  return MOBA_OK;
+}
+
+}  // namespace moba
+
+extern "C" int moba_paged_layout(moba_paged* c) {
+  using namespace moba;
+  Paged p;
+  const int st = check_attention(c, &p);
+  if (st) return st;
+  c->workspace_bytes = static_cast<int64_t>(plan_of(*c).total);
+  return MOBA_OK;
+}
+
+extern "C" int moba_paged_gate(const moba_paged* c, void* stream) {
+  using namespace moba;
+  GateArgs a;
+  int st = check_attention(c, &a.p);
+  if (st) return st;
+  if (!aligned(c->q) || !aligned(c->kbar) || !c->block_idx)
+    return fail(MOBA_ERR_INVALID, "null or unaligned pointer");
+  const PagedPlan pl = plan_of(*c);
+  st = check_workspace(c, pl.total);
+  if (st) return st;
+  a.q = c->q;
+  a.kbar = c->kbar;
+  a.keys = static_cast<uint32_t*>(c->workspace);
+  a.block_idx = c->block_idx;
+  a.h_q = static_cast<int>(c->h_q);
+  a.h_kv = static_cast<int>(c->h_kv);
+  a.slots = static_cast<int>(c->slots);
+  a.take = static_cast<int>(c->take);
+  a.current = c->always_current != 0;
+  hipStream_t s = as_stream(stream);
+  for (int64_t t0 = 0; t0 < c->tokens; t0 += pl.slice) {
+    a.tok0 = static_cast<int32_t>(t0);
+    a.slice = static_cast<int32_t>(c->tokens - t0 < pl.slice ? c->tokens - t0 : pl.slice);
+    st = MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
+      auto go = [&](auto lpr) {
+        constexpr int LPR = decltype(lpr)::value;
+        const int64_t tiles = cdiv(c->table_width, kScoreThreads / LPR * kScoreRows);
+        if (tiles > 65535) return fail(MOBA_ERR_UNSUPPORTED, "block table too wide");
+        hipLaunchKernelGGL((score_kernel<T, LPR>),
+                           dim3(static_cast<unsigned>(a.slice * c->h_kv), static_cast<unsigned>(tiles)),
+                           dim3(kScoreThreads), 0, s, a);
+        return check_launch("moba_paged_gate (scores)");
+      };
+      if (c->take == 0) return static_cast<int>(MOBA_OK);
+      switch (c->head_dim) {
+        case 64: return go(std::integral_constant<int, 4>{});
+        case 128: return go(std::integral_constant<int, 8>{});
+        default: return go(std::integral_constant<int, 16>{});
+      }
+    });
+    if (st) return st;
+    const dim3 grid(static_cast<unsigned>(cdiv(a.slice * c->h_q, 4)));
+    if (c->take <= 8) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(256), 0, s, a);
+    else if (c->take <= 16) hipLaunchKernelGGL(select_kernel<16>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(select_kernel<32>, grid, dim3(256), 0, s, a);
+    st = check_launch("moba_paged_gate (select)");
+    if (st) return st;
+  }
+  return MOBA_OK;
+}
+
+extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
+  using namespace moba;
+  RowArgs a;
+  int st = check_attention(c, &a.p);
+  if (st) return st;
+  if (!aligned(c->q) || !aligned(c->k) || !aligned(c->v) || !aligned(c->out) || !c->block_idx)
+    return fail(MOBA_ERR_INVALID, "null or unaligned pointer");
+  const PagedPlan pl = plan_of(*c);
+  st = check_workspace(c, pl.total);
+  if (st) return st;
+  a.q = c->q;
+  a.k = c->k;
+  a.v = c->v;
+  a.block_idx = c->block_idx;
+  a.out = c->out;
+  a.lse = c->lse;
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.keys);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.keys + pl.ml);
+  a.h_q = static_cast<int>(c->h_q);
+  a.h_kv = static_cast<int>(c->h_kv);
+  a.slots = static_cast<int>(c->slots);
+  a.splits = static_cast<int>(pl.splits);
+  a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(c->head_dim)));
+  hipStream_t s = as_stream(stream);
+  const int64_t rows = c->tokens * c->h_q;
+  return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
+    auto go = [&](auto dim) {
+      constexpr int D = decltype(dim)::value;
+      hipLaunchKernelGGL((attend_rows_kernel<T, D>),
+                         dim3(static_cast<unsigned>(rows), static_cast<unsigned>(a.splits)),
+                         dim3(64 * kRowWaves), 0, s, a);
+      int rc = check_launch("moba_paged_attend");
+      if (rc || a.splits == 1) return rc;
+      hipLaunchKernelGGL((merge_rows_kernel<T, D>), dim3(static_cast<unsigned>(rows)), dim3(64), 0, s, a);
+      return check_launch("moba_paged_attend (merge)");
+    };
+    switch (c->head_dim) {
+      case 64: return go(std::integral_constant<int, 64>{});
+      case 128: return go(std::integral_constant<int, 128>{});
+      default: return go(std::integral_constant<int, 256>{});
+    }
+  });
+}
+
+extern "C" int moba_paged_attention(const moba_paged* c, void* stream) {
+  const int st = moba_paged_gate(c, stream);
+  return st ? st : moba_paged_attend(c, stream);
+}

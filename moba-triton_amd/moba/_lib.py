@@ -26,6 +26,7 @@ DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 # Every symbol declared in include/moba_hip.h, with its ctypes signature.
 _P, _I, _L, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_D = ctypes.c_double
 SIGNATURES = {
     "moba_abi_version": (_I, []),
     "moba_last_error": (ctypes.c_char_p, []),
@@ -53,6 +54,15 @@ SIGNATURES = {
     "moba_step_layout": (_I, [_P]),
     "moba_forward_step": (_I, [_P, _P]),
     "moba_backward_step": (_I, [_P, _P]),
+    "moba_norm_rotate": (_I, [_P] * 9 + [_L] * 5 + [_P, _L, _L, _I, _D, _I, _I, _P]),
+    "moba_norm_rotate_bwd_workspace_size": (_Z, [_L]),
+    "moba_norm_rotate_bwd": (_I, [_P] * 13 + [_L] * 5 + [_P, _L, _L, _I, _D, _I, _I, _P, _Z, _P]),
+    "moba_append_tokens": (_I, [_P] * 9 + [_L, _L, _I, _D, _I, _P]),
+    "moba_paged_layout": (_I, [_P]),
+    "moba_paged_gate": (_I, [_P, _P]),
+    "moba_paged_attend": (_I, [_P, _P]),
+    "moba_paged_attention": (_I, [_P, _P]),
+    "moba_copy_pages": (_I, [_P] * 5 + [_L, _I] + [_L] * 5 + [_I, _P]),
 }
 
 
@@ -65,6 +75,16 @@ class Step(ctypes.Structure):
         "n_blocks", "saved_bytes", "forward_temp", "backward_temp", "failed_stage")] +
         [(n, _P) for n in ("q", "k", "v", "cu_seqlens", "out", "saved", "temp", "dout", "dq", "dk",
                            "dv")])
+
+
+class Paged(ctypes.Structure):
+    """`moba_paged` of include/moba_hip.h."""
+
+    _fields_ = ([(n, _L) for n in (
+        "tokens", "seqs", "h_q", "h_kv", "head_dim", "block_size", "table_width", "n_pages", "dtype",
+        "even", "slots", "take", "always_current", "workspace_bytes")] +
+        [(n, _P) for n in ("q", "k", "v", "kbar", "block_table", "seq_lens", "cu_seqlens",
+                           "block_idx", "out", "lse", "workspace")])
 
 
 # Entry point behind each value of Step.failed_stage.
@@ -102,11 +122,31 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} has ABI version {version}, these bindings expect "
             f"{ABI_VERSION}; rebuild it")
     for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:  # built before the entry point was added
+            raise LibraryMissing(f"{LIB_PATH} has no {name}; rebuild it")
         fn.restype = res
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+class on_device:
+    """Launches inside go to `device`, whichever is the current one."""
+
+    def __init__(self, device: torch.device):
+        index = device.index
+        self._guard = None
+        if index is not None and index != torch.cuda.current_device():
+            self._guard = torch.cuda.device(index)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
 
 
 def available() -> tuple[bool, str]:
@@ -174,6 +214,16 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
     if dev is None:
         raise RuntimeError("no tensor given")
     return dev
+
+
+def aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself where its rows (the last axis) can be read in 16-byte pieces
+    at its strides, else a contiguous copy."""
+    piece = 16 // t.element_size()
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and \
+            all(s % piece == 0 for s in t.stride()[:-1]):
+        return t
+    return aligned_contiguous(t)
 
 
 def aligned_contiguous(t: torch.Tensor) -> torch.Tensor:
