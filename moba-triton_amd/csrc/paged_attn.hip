@@ -7,6 +7,7 @@
 // never ranks. Attention: softmax(q . k / sqrt D) v over the chosen blocks'
 // keys up to the token's own position.
 #include "paged.h"
+#include "paged_chunk.h"
 #include "rotary.h"
 
 namespace moba {
@@ -355,6 +356,7 @@ PagedPlan plan_of(const moba_paged& c) {
   pl.ml = align256(sizeof(float) * 2 * parts);
   pl.o = align256(sizeof(float) * c.head_dim * parts);
   pl.total = pl.keys + pl.ml + pl.o;
+  if (chunk_takes(c)) pl.total = pl.keys + chunk_plan(c).total;
   return pl;
 }
 
@@ -366,8 +368,8 @@ int check_attention(const moba_paged* c, Paged* p) {
   if (c->take > MOBA_PAGED_MAX_TAKE)
     return fail(MOBA_ERR_UNSUPPORTED, "more than " + std::to_string(MOBA_PAGED_MAX_TAKE) +
                                           " past blocks per query");
-  if (c->tokens * c->h_q > (int64_t(1) << 31) - 1)
-    return fail(MOBA_ERR_UNSUPPORTED, "more than 2^31 - 1 query rows");
+  if (c->tokens * c->h_q > ((int64_t(1) << 31) - 1) / c->slots)
+    return fail(MOBA_ERR_UNSUPPORTED, "more than 2^31 - 1 (query, slot) entries");
   return MOBA_OK;
 }
 
@@ -496,6 +498,7 @@ extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
   a.splits = static_cast<int>(pl.splits);
   a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(c->head_dim)));
   hipStream_t s = as_stream(stream);
+  if (chunk_takes(*c)) return chunk_attend(*c, a.p, static_cast<char*>(c->workspace) + pl.keys, s);
   const int64_t rows = c->tokens * c->h_q;
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
     auto go = [&](auto dim) {
