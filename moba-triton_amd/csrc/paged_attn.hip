@@ -1,158 +1,15 @@
-// MoBA attention of new tokens over a paged cache.
-//
-// Gate: score(j) = T(float32(q . kbar_j)) for the strictly past blocks j < own
-// = position / block, the product exact (float64); the `take` best by (score
-// desc, block id asc), ids ascending, the own block last, -1 padding: the
-// rules of gate.hip. A block without a page (a table entry outside the cache)
-// never ranks. Attention: softmax(q . k / sqrt D) v over the chosen blocks'
-// keys up to the token's own position.
+// MoBA attention of new tokens over a paged cache: softmax(q . k / sqrt D) v
+// over the keys, up to the token's own position, of the blocks that
+// paged_gate.hip chose. Here each query by itself, every type and size;
+// paged_chunk.hip goes block by block where many queries share blocks.
 #include "paged.h"
 #include "paged_chunk.h"
+#include "paged_gate.h"
 #include "rotary.h"
 
 namespace moba {
 
 namespace {
-
-struct GateArgs {
-  Paged p;
-  const void* q;      // [tokens, h_q, D]
-  const void* kbar;   // [pages, h_kv, D]
-  uint32_t* keys;     // [slice tokens, h_q, width]
-  int32_t* block_idx; // [tokens, h_q, slots]
-  int32_t tok0, slice;  // tokens [tok0, tok0 + slice) of this launch
-  int h_q, h_kv, slots, take, current;
-};
-
-// A rounded score as an integer in the order of the scores, 0 for what never
-// ranks (-inf, NaN).
-__device__ inline uint32_t score_key(float rounded) {
-  const uint32_t u = f2u(rounded + 0.f);
-  const uint32_t o = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
-  return o > 0x007fffffu && o <= 0xff800000u ? o : 0u;
-}
-
-// Scores of one token's query heads of one kv head against a run of its past
-// blocks: a block's representative belongs to D / 16 lanes, which hold it in
-// float64 for the heads of the group.
-constexpr int kScoreThreads = 256;
-constexpr int kScoreRows = 4;  // blocks per lane group
-template <typename T, int LPR>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(GateArgs a) {
-  constexpr int D = 16 * LPR;
-  constexpr int G = kScoreThreads / LPR;
-  const int32_t local = blockIdx.x / a.h_kv;
-  const int hk = blockIdx.x % a.h_kv;
-  const TokenAt at = locate(a.p, a.tok0 + local);
-  if (at.pos < 0) return;
-  const int32_t own = at.pos / a.p.block;
-  const int32_t past = own < a.p.width ? own : a.p.width;
-  const int32_t j0 = blockIdx.y * (G * kScoreRows);
-  if (j0 >= past) return;
-  const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
-  const RotLane rl = rot_lane(lane, 0, 0);
-  const int group = a.h_q / a.h_kv;
-  const T* q = static_cast<const T*>(a.q) +
-               (static_cast<int64_t>(a.tok0 + local) * a.h_q + hk * group) * D;
-  for (int i = 0; i < kScoreRows; ++i) {
-    const int32_t j = j0 + i * G + g;
-    if (j >= past) break;
-    const int32_t page = page_of(a.p, at.seq, j);
-    double kd[16];
-    {
-      RawRow<T> raw;
-      raw.load(static_cast<const T*>(a.kbar) +
-                   (static_cast<int64_t>(page < 0 ? 0 : page) * a.h_kv + hk) * D, rl);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) kd[e] = static_cast<double>(raw.element(e));
-    }
-    for (int h = 0; h < group; ++h) {
-      RawRow<T> raw;
-      raw.load(q + h * D, rl);
-      double t = 0.0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) t = fma(static_cast<double>(raw.element(e)), kd[e], t);
-#pragma unroll
-      for (int off = 1; off < LPR; off <<= 1) t += __shfl_xor(t, off);
-      if (lane == 0)
-        a.keys[(static_cast<int64_t>(local) * a.h_q + hk * group + h) * a.p.width + j] =
-            page < 0 ? 0u : score_key(Elem<T>::round(static_cast<float>(t)));
-    }
-  }
-}
-
-// The `take` best of a query's scores: one wave per (token, query head). Each
-// lane keeps the best TM of every 64th block, the lanes' lists meet in six
-// exchanges, each the best TM of two sorted lists.
-template <int TM>
-__global__ void __launch_bounds__(256) select_kernel(GateArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= static_cast<int64_t>(a.slice) * a.h_q) return;
-  const int lane = threadIdx.x & 63;
-  const TokenAt at = locate(a.p, a.tok0 + static_cast<int32_t>(row / a.h_q));
-  int32_t* out = a.block_idx + (static_cast<int64_t>(a.tok0) * a.h_q + row) * a.slots;
-  if (at.pos < 0) {
-    for (int i = lane; i < a.slots; i += 64) out[i] = -1;
-    return;
-  }
-  const int32_t own = at.pos / a.p.block;
-  const int32_t past = own < a.p.width ? own : a.p.width;
-  const uint32_t* keys = a.keys + row * a.p.width;
-  // (score, id) in one word, larger first: equal scores go to the lower id.
-  uint64_t best[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) best[i] = 0;
-  for (int32_t j = lane; j < past; j += 64) {
-    const uint32_t key = keys[j];
-    uint64_t x = key ? (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(j)) : 0;
-    if (x > best[TM - 1]) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const bool up = x > best[i];
-        const uint64_t t = up ? best[i] : x;
-        best[i] = up ? x : best[i];
-        x = t;
-      }
-    }
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    uint64_t other[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) other[i] = __shfl_xor(best[i], off);
-    // The larger of entry i and the other list's entry TM - 1 - i: the best
-    // TM of both, in an order that log2 TM exchange stages sort.
-#pragma unroll
-    for (int i = 0; i < TM; ++i) best[i] = best[i] > other[TM - 1 - i] ? best[i] : other[TM - 1 - i];
-#pragma unroll
-    for (int st = TM / 2; st > 0; st >>= 1)
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if ((i & st) == 0) {
-          const uint64_t x = best[i], y = best[i + st];
-          best[i] = x > y ? x : y;
-          best[i + st] = x > y ? y : x;
-        }
-  }
-  // Lane i takes entry i, and its place among the chosen ids.
-  uint32_t id = 0xffffffffu;
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-    if (i == lane && i < a.take && best[i]) id = 0xffffffffu - static_cast<uint32_t>(best[i]);
-  const uint64_t live = __ballot(id != 0xffffffffu);
-  int place = 0;
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const uint32_t other = __shfl(id, i);
-    place += other < id ? 1 : 0;
-  }
-  int n = __popcll(live);
-  if (id != 0xffffffffu) out[place] = static_cast<int32_t>(id);
-  const bool cur = a.current && page_of(a.p, at.seq, own) >= 0;
-  if (cur && lane == 0) out[n] = own;
-  n += cur;
-  for (int i = n + lane; i < a.slots; i += 64) out[i] = -1;
-}
 
 struct RowArgs {
   Paged p;
@@ -331,9 +188,8 @@ __global__ void __launch_bounds__(64) merge_rows_kernel(RowArgs a) {
 
 // How a call is cut up, and its workspace.
 struct PagedPlan {
-  int64_t slice;   // tokens per gate launch
   int64_t splits;  // parts of a query's chosen blocks
-  size_t keys, ml, o, total;
+  size_t ml, o, total;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -343,20 +199,18 @@ int64_t run_keys(int64_t D, int dtype) { return 64 * 8 / (D / (dtype == MOBA_FP3
 
 PagedPlan plan_of(const moba_paged& c) {
   PagedPlan pl;
-  const int64_t per_token = c.h_q * c.table_width;
-  pl.slice = (int64_t(1) << 24) / per_token;
-  pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
   const int64_t rows = c.tokens * c.h_q;
   const int64_t units = c.slots * cdiv(c.block_size, run_keys(c.head_dim, static_cast<int>(c.dtype)));
   int64_t splits = cdiv(2048, rows * kRowWaves);
   const int64_t most = cdiv(units, kRowWaves);
   pl.splits = splits < most ? splits : most;
-  pl.keys = align256(sizeof(uint32_t) * static_cast<size_t>(pl.slice * per_token));
   const size_t parts = pl.splits > 1 ? static_cast<size_t>(rows * pl.splits) : 0;
   pl.ml = align256(sizeof(float) * 2 * parts);
   pl.o = align256(sizeof(float) * c.head_dim * parts);
-  pl.total = pl.keys + pl.ml + pl.o;
-  if (chunk_takes(c)) pl.total = pl.keys + chunk_plan(c).total;
+  // The gate's scratch is free again when the attention starts.
+  const size_t attend = chunk_takes(c) ? chunk_plan(c).total : pl.ml + pl.o;
+  const size_t gate = gate_workspace(c);
+  pl.total = attend > gate ? attend : gate;
   return pl;
 }
 
@@ -423,56 +277,19 @@ extern "C" int moba_paged_layout(moba_paged* c) {
   return MOBA_OK;
 }
 
-extern "C" int moba_paged_gate(const moba_paged* c, void* stream) {
+static int run_gate(const moba_paged* c, bool all_rows, void* stream) {
   using namespace moba;
-  GateArgs a;
-  int st = check_attention(c, &a.p);
+  Paged p;
+  int st = check_attention(c, &p);
   if (st) return st;
   if (!aligned(c->q) || !aligned(c->kbar) || !c->block_idx)
     return fail(MOBA_ERR_INVALID, "null or unaligned pointer");
-  const PagedPlan pl = plan_of(*c);
-  st = check_workspace(c, pl.total);
+  st = check_workspace(c, plan_of(*c).total);
   if (st) return st;
-  a.q = c->q;
-  a.kbar = c->kbar;
-  a.keys = static_cast<uint32_t*>(c->workspace);
-  a.block_idx = c->block_idx;
-  a.h_q = static_cast<int>(c->h_q);
-  a.h_kv = static_cast<int>(c->h_kv);
-  a.slots = static_cast<int>(c->slots);
-  a.take = static_cast<int>(c->take);
-  a.current = c->always_current != 0;
-  hipStream_t s = as_stream(stream);
-  for (int64_t t0 = 0; t0 < c->tokens; t0 += pl.slice) {
-    a.tok0 = static_cast<int32_t>(t0);
-    a.slice = static_cast<int32_t>(c->tokens - t0 < pl.slice ? c->tokens - t0 : pl.slice);
-    st = MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
-      auto go = [&](auto lpr) {
-        constexpr int LPR = decltype(lpr)::value;
-        const int64_t tiles = cdiv(c->table_width, kScoreThreads / LPR * kScoreRows);
-        if (tiles > 65535) return fail(MOBA_ERR_UNSUPPORTED, "block table too wide");
-        hipLaunchKernelGGL((score_kernel<T, LPR>),
-                           dim3(static_cast<unsigned>(a.slice * c->h_kv), static_cast<unsigned>(tiles)),
-                           dim3(kScoreThreads), 0, s, a);
-        return check_launch("moba_paged_gate (scores)");
-      };
-      if (c->take == 0) return static_cast<int>(MOBA_OK);
-      switch (c->head_dim) {
-        case 64: return go(std::integral_constant<int, 4>{});
-        case 128: return go(std::integral_constant<int, 8>{});
-        default: return go(std::integral_constant<int, 16>{});
-      }
-    });
-    if (st) return st;
-    const dim3 grid(static_cast<unsigned>(cdiv(a.slice * c->h_q, 4)));
-    if (c->take <= 8) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(256), 0, s, a);
-    else if (c->take <= 16) hipLaunchKernelGGL(select_kernel<16>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(select_kernel<32>, grid, dim3(256), 0, s, a);
-    st = check_launch("moba_paged_gate (select)");
-    if (st) return st;
-  }
-  return MOBA_OK;
+  return gate_run(*c, p, c->workspace, all_rows, as_stream(stream));
 }
+
+extern "C" int moba_paged_gate(const moba_paged* c, void* stream) { return run_gate(c, true, stream); }
 
 extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
   using namespace moba;
@@ -490,15 +307,15 @@ extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
   a.block_idx = c->block_idx;
   a.out = c->out;
   a.lse = c->lse;
-  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.keys);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.keys + pl.ml);
+  a.part_ml = static_cast<float*>(c->workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.ml);
   a.h_q = static_cast<int>(c->h_q);
   a.h_kv = static_cast<int>(c->h_kv);
   a.slots = static_cast<int>(c->slots);
   a.splits = static_cast<int>(pl.splits);
   a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(c->head_dim)));
   hipStream_t s = as_stream(stream);
-  if (chunk_takes(*c)) return chunk_attend(*c, a.p, static_cast<char*>(c->workspace) + pl.keys, s);
+  if (chunk_takes(*c)) return chunk_attend(*c, a.p, c->workspace, s);
   const int64_t rows = c->tokens * c->h_q;
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
     auto go = [&](auto dim) {
@@ -520,6 +337,6 @@ extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
 }
 
 extern "C" int moba_paged_attention(const moba_paged* c, void* stream) {
-  const int st = moba_paged_gate(c, stream);
+  const int st = run_gate(c, false, stream);
   return st ? st : moba_paged_attend(c, stream);
 }

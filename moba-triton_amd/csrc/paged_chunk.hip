@@ -16,6 +16,8 @@
 // row. Entries of a column stand in no particular order; nothing depends on it.
 #include "paged_chunk.h"
 
+#include "paged_gate.h"
+
 namespace moba {
 
 namespace {
@@ -46,43 +48,6 @@ template <> struct Unit<f16_t> {
 
 // Entries of a work item: one group of 32 for each of the four waves.
 constexpr int kItem = 128;
-
-// The part-th run of a sequence's new tokens, at most `size` of them, inside
-// the tokens [t0, t1). Parts are counted 64 sequences at a time.
-struct Part {
-  int32_t seq, begin, end;  // tokens; seq -1: no such part
-  int32_t first, total;     // the sequence's parts: index of its first, their number
-};
-
-__device__ inline Part find_part(const Paged& p, int32_t t0, int32_t t1, int32_t size, int32_t part) {
-  const int lane = threadIdx.x & 63;
-  int32_t before = 0;
-  for (int32_t base = 0; base < p.seqs; base += 64) {
-    NewTokens r{0, 0, 0};
-    if (base + lane < p.seqs) r = new_tokens(p, base + lane);
-    const int32_t lo = max(r.first, t0), hi = min(r.first + r.n, t1);
-    const int32_t mine = hi > lo ? (hi - lo + size - 1) / size : 0;
-    int32_t upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int32_t y = __shfl_up(upto, off);
-      if (lane >= off) upto += y;
-    }
-    const uint64_t past = __ballot(before + upto > part);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      Part out;
-      out.total = __shfl(mine, l);
-      out.first = before + __shfl(upto, l) - out.total;
-      out.seq = base + l;
-      out.begin = __shfl(lo, l) + (part - out.first) * size;
-      out.end = min(out.begin + size, __shfl(hi, l));
-      return out;
-    }
-    before += __shfl(upto, 63);
-  }
-  return Part{-1, 0, 0, 0, 0};
-}
 
 // The block an entry of sequence `seq` attends to, or -1: padding, a block
 // without a page or behind the sequence's last token.

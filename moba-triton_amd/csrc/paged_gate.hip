@@ -1,0 +1,624 @@
+// Which blocks new tokens attend to over a paged cache.
+//
+// score(j) = T(float32(q . kbar_j)) for the strictly past blocks j < own =
+// position / block, the product exact; the `take` best by (score desc, block
+// id asc), ids ascending, the own block last, -1 padding: the rules of
+// gate.hip. A block without a page (a table entry outside the cache) never
+// ranks, nor do scores of -inf and NaN.
+//
+// * score_kernel, select_kernel: every type and size, and few queries. All
+//   scores in float64, over the whole chip, then one wave per query.
+// * tiles_kernel: 16-bit types, many queries (below).
+#include "paged_gate.h"
+
+#include <type_traits>
+
+#include "rotary.h"
+
+namespace moba {
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct GateArgs {
+  Paged p;
+  const void* q;      // [tokens, h_q, D]
+  const void* kbar;   // [pages, h_kv, D]
+  uint32_t* keys;     // score_kernel: [slice tokens, h_q, width]
+  uint32_t* norms;    // tiles_kernel: [seqs, h_kv, kNormParts] float bits
+  int32_t* block_idx; // [tokens, h_q, slots]
+  int32_t tok0, slice;  // tokens [tok0, tok0 + slice) of this launch
+  int h_q, h_kv, slots, take, current;
+  int tile_tokens;    // tiles_kernel: tokens per workgroup
+};
+
+// A rounded score as an integer in the order of the scores, 0 for what never
+// ranks (-inf, NaN).
+__device__ inline uint32_t score_key(float rounded) {
+  const uint32_t u = f2u(rounded + 0.f);
+  const uint32_t o = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return o > 0x007fffffu && o <= 0xff800000u ? o : 0u;
+}
+
+// A wave's best TM entries: (score, id) in one word, larger first, so that
+// equal scores go to the lower id; 0 for none. Each lane fills its own list.
+template <int TM>
+struct WaveBest {
+  uint64_t best[TM];
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) best[i] = 0;
+  }
+  __device__ void add(uint32_t key, int32_t j) {
+    uint64_t x = key ? (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(j)) : 0;
+    if (x > best[TM - 1]) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const bool up = x > best[i];
+        const uint64_t t = up ? best[i] : x;
+        best[i] = up ? x : best[i];
+        x = t;
+      }
+    }
+  }
+  // The lanes' lists meet in six exchanges. The larger of entry i and the
+  // other list's entry TM - 1 - i: the best TM of both, in an order that log2
+  // TM exchange stages sort.
+  __device__ void meet() {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      uint64_t other[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) other[i] = __shfl_xor(best[i], off);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) best[i] = best[i] > other[TM - 1 - i] ? best[i] : other[TM - 1 - i];
+#pragma unroll
+      for (int st = TM / 2; st > 0; st >>= 1)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          if ((i & st) == 0) {
+            const uint64_t x = best[i], y = best[i + st];
+            best[i] = x > y ? x : y;
+            best[i + st] = x > y ? y : x;
+          }
+    }
+  }
+  // Lane i takes entry i, and its place among the chosen ids; own >= 0 goes
+  // behind them.
+  __device__ void emit(int take, int32_t own, int slots, int32_t* out) const {
+    const int lane = threadIdx.x & 63;
+    uint32_t id = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      if (i == lane && i < take && best[i]) id = 0xffffffffu - static_cast<uint32_t>(best[i]);
+    int n = __popcll(__ballot(id != 0xffffffffu));
+    int place = 0;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) place += static_cast<uint32_t>(__shfl(id, i)) < id ? 1 : 0;
+    if (id != 0xffffffffu) out[place] = static_cast<int32_t>(id);
+    if (own >= 0 && lane == 0) out[n] = own;
+    n += own >= 0;
+    for (int i = n + lane; i < slots; i += 64) out[i] = -1;
+  }
+};
+
+// The own block where it counts, else -1.
+__device__ inline int32_t own_entry(const GateArgs& a, int32_t seq, int32_t own) {
+  return a.current && page_of(a.p, seq, own) >= 0 ? own : -1;
+}
+
+// Scores of one token's query heads of one kv head against a run of its past
+// blocks: a block's representative belongs to D / 16 lanes, which hold it in
+// float64 for the heads of the group.
+constexpr int kScoreThreads = 256;
+constexpr int kScoreRows = 4;  // blocks per lane group
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kScoreThreads) score_kernel(GateArgs a) {
+  constexpr int D = 16 * LPR;
+  constexpr int G = kScoreThreads / LPR;
+  const int32_t local = blockIdx.x / a.h_kv;
+  const int hk = blockIdx.x % a.h_kv;
+  const TokenAt at = locate(a.p, a.tok0 + local);
+  if (at.pos < 0) return;
+  const int32_t own = at.pos / a.p.block;
+  const int32_t past = own < a.p.width ? own : a.p.width;
+  const int32_t j0 = blockIdx.y * (G * kScoreRows);
+  if (j0 >= past) return;
+  const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
+  const RotLane rl = rot_lane(lane, 0, 0);
+  const int group = a.h_q / a.h_kv;
+  const T* q = static_cast<const T*>(a.q) +
+               (static_cast<int64_t>(a.tok0 + local) * a.h_q + hk * group) * D;
+  for (int i = 0; i < kScoreRows; ++i) {
+    const int32_t j = j0 + i * G + g;
+    if (j >= past) break;
+    const int32_t page = page_of(a.p, at.seq, j);
+    double kd[16];
+    {
+      RawRow<T> raw;
+      raw.load(static_cast<const T*>(a.kbar) +
+                   (static_cast<int64_t>(page < 0 ? 0 : page) * a.h_kv + hk) * D, rl);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) kd[e] = static_cast<double>(raw.element(e));
+    }
+    for (int h = 0; h < group; ++h) {
+      RawRow<T> raw;
+      raw.load(q + h * D, rl);
+      double t = 0.0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t = fma(static_cast<double>(raw.element(e)), kd[e], t);
+#pragma unroll
+      for (int off = 1; off < LPR; off <<= 1) t += __shfl_xor(t, off);
+      if (lane == 0)
+        a.keys[(static_cast<int64_t>(local) * a.h_q + hk * group + h) * a.p.width + j] =
+            page < 0 ? 0u : score_key(Elem<T>::round(static_cast<float>(t)));
+    }
+  }
+}
+
+// The `take` best of a query's scores: one wave per (token, query head), each
+// lane every 64th block.
+template <int TM>
+__global__ void __launch_bounds__(256) select_kernel(GateArgs a) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= static_cast<int64_t>(a.slice) * a.h_q) return;
+  const int lane = threadIdx.x & 63;
+  const TokenAt at = locate(a.p, a.tok0 + static_cast<int32_t>(row / a.h_q));
+  int32_t* out = a.block_idx + (static_cast<int64_t>(a.tok0) * a.h_q + row) * a.slots;
+  if (at.pos < 0) {
+    for (int i = lane; i < a.slots; i += 64) out[i] = -1;
+    return;
+  }
+  const int32_t own = at.pos / a.p.block;
+  const int32_t past = own < a.p.width ? own : a.p.width;
+  const uint32_t* keys = a.keys + row * a.p.width;
+  WaveBest<TM> list;
+  list.clear();
+  for (int32_t j = lane; j < past && a.take; j += 64) list.add(keys[j], j);
+  list.meet();
+  list.emit(a.take, own_entry(a, at.seq, own), a.slots, out);
+}
+
+// ---------------------------------------------------------------------------
+// Many queries, 16-bit types. A wave holds 32 queries (tokens by the query
+// heads of one kv head), two lanes each; the representatives pass through LDS
+// 64 at a time, and a 32x32x16 MFMA chain leaves each lane 16 approximate
+// scores of its query. |approximate - exact| <= E: the products are exact in
+// float32, D additions round by at most a unit of the last place each
+// (truncation included) of sums of at most |q| |kbar|; and what the unit may
+// flush below the normal range.
+//
+// Each lane keeps the best M of its blocks by (largest key the score can
+// have, id), a key being the score rounded to the type. An entry whose
+// smallest key is the same is certain, the others are marked. At the end a
+// lane forms the exact scores of its marked entries, as far down as `take`
+// certain ones do not stand above them, and the two lists are ranked. What
+// left a list has no larger key than its last entry had, so the result stands
+// where the last chosen entry ranks no lower than both lists' last; the other
+// queries (constructed ties, infinities, NaN) score every block exactly.
+//
+// Bound by the list work: [2048 tokens, 32/8 heads of 128, 1008 blocks] is 17
+// GFLOP of products, tens of instructions per kept score.
+constexpr int kNormParts = 16;
+
+template <typename T> struct GateUnit;
+template <> struct GateUnit<bf16_t> {
+  typedef bf16x8_t vec;
+  static constexpr float kFlush = 1.2e-38f;  // inputs below it may count as 0
+  static constexpr float kLowest = -3.3961514e38f;  // rounds to -inf, as all below it
+  __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // x rounded to the type, its bits in the upper half.
+  __device__ static uint32_t bits(float x) {
+    return f2u(static_cast<float>(static_cast<__bf16>(x)) + 0.f);
+  }
+  // The value of a rounded score's ordered bits.
+  __device__ static float value(uint32_t upper) { return u2f(upper); }
+};
+template <> struct GateUnit<f16_t> {
+  typedef f16x8_t vec;
+  static constexpr float kFlush = 6.2e-5f;
+  static constexpr float kLowest = -65520.f;
+  __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static uint32_t bits(float x) {
+    const _Float16 r = static_cast<_Float16>(x) + static_cast<_Float16>(0);
+    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, r)) << 16;
+  }
+  __device__ static float value(uint32_t upper) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(upper >> 16)));
+  }
+};
+
+// Order of 16-bit floats in the upper half of a word, and back.
+__device__ inline uint32_t ordered(uint32_t u) {
+  return (u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u)) & 0xffff0000u;
+}
+__device__ inline uint32_t unordered(uint32_t o) {
+  return (o & 0x80000000u ? o ^ 0x80000000u : ~o) & 0xffff0000u;
+}
+
+__device__ inline uint32_t med3(uint32_t a, uint32_t b, uint32_t c) {
+  return max(min(a, b), min(max(a, b), c));
+}
+
+// The largest |kbar| of every (sequence, kv head)'s past blocks, in kNormParts
+// parts, as float bits (NaN largest). grid (seqs * h_kv, kNormParts).
+template <typename T, int LPR>
+__global__ void __launch_bounds__(256) norm_kernel(GateArgs a) {
+  constexpr int D = 16 * LPR;
+  __shared__ uint32_t s_best[4];
+  const int32_t seq = blockIdx.x / a.h_kv;
+  const int hk = blockIdx.x % a.h_kv;
+  const NewTokens r = new_tokens(a.p, seq);
+  const int32_t past = r.n ? min((r.len - 1) / a.p.block, a.p.width) : 0;
+  const RotLane rl = rot_lane(threadIdx.x % LPR, 0, 0);
+  uint32_t best = 0;
+  for (int32_t j = blockIdx.y * (256 / LPR) + threadIdx.x / LPR; j < past; j += kNormParts * (256 / LPR)) {
+    const int32_t page = page_of(a.p, seq, j);
+    if (page < 0) continue;
+    RawRow<T> raw;
+    raw.load(static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D, rl);
+    float v[16];
+    raw.widen(v);
+    best = max(best, f2u(sqrtf(row_sum<LPR>(square_sum(v)))) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) best = max(best, static_cast<uint32_t>(__shfl_xor(static_cast<int>(best), off)));
+  if ((threadIdx.x & 63) == 0) s_best[threadIdx.x >> 6] = best;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.norms[static_cast<int64_t>(blockIdx.x) * kNormParts + blockIdx.y] =
+        max(max(s_best[0], s_best[1]), max(s_best[2], s_best[3]));
+}
+
+// Exact key of one block, by one lane.
+template <typename T, int D>
+__device__ inline uint32_t exact_key(const T* q, const T* kb) {
+  double t = 0.0;
+  for (int d = 0; d < D; d += 8) {
+    const u32x4 qa = *reinterpret_cast<const u32x4*>(q + d);
+    const u32x4 ka = *reinterpret_cast<const u32x4*>(kb + d);
+    const T* qe = reinterpret_cast<const T*>(&qa);
+    const T* ke = reinterpret_cast<const T*>(&ka);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      t = fma(static_cast<double>(Elem<T>::load(qe, e)), static_cast<double>(Elem<T>::load(ke, e)), t);
+  }
+  return score_key(Elem<T>::round(static_cast<float>(t)));
+}
+
+// A query's blocks all scored exactly, by one wave.
+template <typename T, int D, int TM>
+__device__ __attribute__((noinline)) void exact_query(const GateArgs& a, int32_t seq, int32_t own, int hk,
+                                                      const T* q, int32_t* out) {
+  WaveBest<TM> list;
+  list.clear();
+  const int32_t past = min(own, a.p.width);
+  for (int32_t j = threadIdx.x & 63; j < past; j += 64) {
+    const int32_t page = page_of(a.p, seq, j);
+    if (page >= 0)
+      list.add(exact_key<T, D>(q, static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D), j);
+  }
+  list.meet();
+  list.emit(a.take, own_entry(a, seq, own), a.slots, out);
+}
+
+template <typename T, int D, int M, int TM>
+__global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
+  using U = GateUnit<T>;
+  using V8 = typename U::vec;
+  constexpr int RQ = D / 8;     // 16-byte pieces per row
+  constexpr int ROWS = 64;      // representatives per stage
+  constexpr int KS = D / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t rows[2][ROWS * D];
+  __shared__ int32_t s_page[2][ROWS];
+  __shared__ uint64_t s_valid[4];
+  const Part pt = find_part(a.p, 0, a.p.tokens, a.tile_tokens, blockIdx.x);
+  if (pt.seq < 0) return;
+  const NewTokens nt = new_tokens(a.p, pt.seq);
+  const int hk = blockIdx.y, group = a.h_q / a.h_kv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int n_rows = (pt.end - pt.begin) * group;
+  const int mine = wave * 32 + (lane & 31);
+  const bool live = mine < n_rows;
+  const bool busy = wave * 32 < n_rows;  // the wave has queries
+  const int32_t tok = pt.begin + (live ? mine : 0) / group;
+  const int64_t qrow = static_cast<int64_t>(tok) * a.h_q + hk * group + (live ? mine : 0) % group;
+  const T* q = static_cast<const T*>(a.q) + qrow * D;
+  const int32_t pos0 = nt.len - nt.n - nt.first;  // a token's position: pos0 + token
+  const int32_t own = (pos0 + tok) / a.p.block;
+  const int32_t past = live ? min(own, a.p.width) : 0;
+  const int32_t horizon = min((pos0 + pt.end - 1) / a.p.block, a.p.width);
+  const int32_t sure = min((pos0 + pt.begin) / a.p.block, a.p.width);  // past for every query here
+  const int stages = (horizon + ROWS - 1) / ROWS;
+
+  V8 bq[KS];
+  float qn = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    bq[k] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(q + 16 * k + 8 * h));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qn = fmaf(static_cast<float>(bq[k][e]), static_cast<float>(bq[k][e]), qn);
+  }
+  qn = sqrtf(qn + __shfl_xor(qn, 32)) * 1.0001f;
+  float kn = 0.f;
+  {
+    uint32_t best = 0;
+    const uint32_t* norms = a.norms + (static_cast<int64_t>(pt.seq) * a.h_kv + hk) * kNormParts;
+#pragma unroll
+    for (int i = 0; i < kNormParts; ++i) best = max(best, norms[i]);
+    kn = u2f(best) * 1.0001f;
+  }
+  // Widened by the rounding of a -+ E itself, with |a| * 2.4e-7 below.
+  const float E = (qn * kn * (D * 0x1p-23f) + U::kFlush * sqrtf(static_cast<float>(D)) * (qn + kn) +
+                   (D + 1) * 1.2e-38f) * 1.001f;
+  const bool bounded = qn * kn < 3e38f && E < 3e38f;  // false for infinities and NaN
+
+  // Pages of stage st, by wave 0: to LDS, with a bit for each that is one.
+  auto page_at = [&](int st) {
+    const int32_t j = st * ROWS + lane;
+    return j < horizon ? page_of(a.p, pt.seq, j) : -1;
+  };
+  auto put_pages = [&](int st, int32_t page) {
+    const uint64_t ok = __ballot(page >= 0);
+    s_page[st & 1][lane] = max(page, 0);
+    if (lane == 0) s_valid[st & 3] = ok;
+  };
+  auto stage = [&](int st) {
+#pragma unroll
+    for (int u = 0; u < ROWS * RQ / 256; ++u) {
+      const int i = u * 256 + tid, row = i / RQ, piece = i % RQ;
+      const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
+      const T* src = static_cast<const T*>(a.kbar) +
+                     (static_cast<int64_t>(s_page[st & 1][row]) * a.h_kv + hk) * D + 8 * (piece ^ swz);
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
+          (__attribute__((address_space(3))) void*)&rows[st & 1][(u * 256 + wave * 64) * 8], 16, 0, 0);
+    }
+  };
+
+  uint32_t key[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) key[i] = 0;
+  float floor_value = U::kLowest;  // scores that round to at most this cannot enter the list
+  if (stages > 0) {
+    if (wave == 0) {
+      put_pages(0, page_at(0));
+      if (stages > 1) put_pages(1, page_at(1));
+    }
+    __syncthreads();
+    stage(0);
+  }
+  for (int st = 0; st < stages; ++st) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int32_t ahead = -1;
+    if (wave == 0 && st + 2 < stages) ahead = page_at(st + 2);
+    if (st + 1 < stages) stage(st + 1);
+    if (busy) {
+      const uint64_t valid = s_valid[st & 3];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int32_t j0 = st * ROWS + half * 32;
+        if (j0 >= horizon) break;
+        floatx16_t s = floatx16_t{};
+        const int row = half * 32 + (lane & 31);
+        const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          s = U::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
+                                                &rows[st & 1][row * D + 8 * ((2 * k + h) ^ swz)])),
+                     bq[k], s);
+        const uint32_t ok = static_cast<uint32_t>(valid >> (32 * half));
+        if (j0 + 32 > sure || ok != 0xffffffffu) {  // some blocks are not for every query
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int o = 8 * (v >> 2) + 4 * h + (v & 3);
+            if (j0 + o >= past || !((ok >> o) & 1u)) s[v] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float x = s[v];
+          const float hi = fmaf(fabsf(x), 2.4e-7f, x) + E;
+          if (hi > floor_value) {
+            const uint32_t top = U::bits(hi);
+            const uint32_t low = U::bits(fmaf(-fabsf(x), 2.4e-7f, x) - E);
+            const uint32_t j = static_cast<uint32_t>(j0 + 8 * (v >> 2) + 4 * h + (v & 3));
+            const uint32_t e = ordered(top) | (0x7fffu - j) << 1 | (top != low ? 1u : 0u);
+#pragma unroll
+            for (int i = M - 1; i > 0; --i) key[i] = med3(key[i - 1], key[i], e);
+            key[0] = max(key[0], e);
+          }
+        }
+        floor_value = key[M - 1] ? U::value(unordered(key[M - 1])) : U::kLowest;
+      }
+    }
+    if (wave == 0 && st + 2 < stages) put_pages(st + 2, ahead);
+  }
+  if (!busy) return;
+
+  const uint32_t last = key[M - 1];
+  bool settled = bounded || past == 0;
+  // Exact scores of marked entries that `take` certain ones do not outrank.
+  int certain = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    if (key[i] & 1u) {
+      if (settled && certain < a.take) {
+        const int32_t j = static_cast<int32_t>(0x7fffu - ((key[i] >> 1) & 0x7fffu));
+        const int32_t page = max(page_of(a.p, pt.seq, j), 0);
+        const uint32_t x = exact_key<T, D>(
+            q, static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D);
+        // The key as a float's order; 16-bit types: the value's own order.
+        key[i] = x ? ordered(U::bits(u2f(x & 0x80000000u ? x ^ 0x80000000u : ~x))) | (key[i] & 0xfffeu) : 0u;
+      }
+    } else if (key[i]) {
+      ++certain;
+    }
+    key[i] &= ~1u;
+  }
+  // Ranks among both lanes' entries.
+  uint32_t other[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) other[i] = static_cast<uint32_t>(__shfl_xor(static_cast<int>(key[i]), 32));
+  uint32_t lowest = 0xffffffffu;  // the lowest chosen entry
+  int n = 0;
+  uint64_t chosen = 0;            // bits of this lane's chosen entries
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    int rank = 0;
+#pragma unroll
+    for (int u = 0; u < M; ++u) rank += (key[u] > key[i]) + (other[u] > key[i]);
+    if (key[i] && rank < a.take) {
+      chosen |= uint64_t(1) << i;
+      lowest = min(lowest, key[i]);
+      ++n;
+    }
+  }
+  n += __shfl_xor(n, 32);
+  lowest = min(lowest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lowest), 32)));
+  const uint32_t out_of = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), 32)));
+  if (out_of && (n < a.take || lowest < (out_of & ~1u))) settled = false;
+
+  // Places in the order of the ids: larger (0x7fff - id) first.
+  int32_t* out = a.block_idx + qrow * a.slots;
+  const uint64_t theirs = __shfl_xor(static_cast<unsigned long long>(chosen), 32);
+  if (settled && live) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      if (!((chosen >> i) & 1u)) continue;
+      const uint32_t id = key[i] & 0xfffeu;
+      int place = 0;
+#pragma unroll
+      for (int u = 0; u < M; ++u)
+        place += (((chosen >> u) & 1u) && (key[u] & 0xfffeu) > id) +
+                 (((theirs >> u) & 1u) && (other[u] & 0xfffeu) > id);
+      out[place] = static_cast<int32_t>(0x7fffu - (id >> 1));
+    }
+    if (h == 0) {
+      const int32_t o = own_entry(a, pt.seq, own);
+      if (o >= 0) out[n++] = o;
+      for (; n < a.slots; ++n) out[n] = -1;
+    }
+  }
+  uint64_t open = __ballot(!settled && live && h == 0);
+  while (open) {
+    const int l = __builtin_ctzll(open);
+    open &= open - 1;
+    const int row = wave * 32 + l;
+    const int32_t t = pt.begin + row / group;
+    const int64_t qr = static_cast<int64_t>(t) * a.h_q + hk * group + row % group;
+    exact_query<T, D, TM>(a, pt.seq, (pos0 + t) / a.p.block, hk, static_cast<const T*>(a.q) + qr * D,
+                          a.block_idx + qr * a.slots);
+  }
+}
+
+// Rows of no sequence: all -1. One wave per token.
+__global__ void __launch_bounds__(64) nobody_kernel(GateArgs a) {
+  if (locate(a.p, blockIdx.x).pos >= 0) return;
+  int32_t* out = a.block_idx + static_cast<int64_t>(blockIdx.x) * a.h_q * a.slots;
+  for (int i = threadIdx.x; i < a.h_q * a.slots; i += 64) out[i] = -1;
+}
+
+bool tiles_take(const moba_paged& c) {
+  return c.dtype != MOBA_FP32 && c.take > 0 && c.table_width < (1 << 15) && c.h_q / c.h_kv <= 128 &&
+         c.h_kv <= 65535 && c.tokens >= 4 * c.seqs;
+}
+
+int64_t score_slice(const moba_paged& c) {
+  const int64_t n = (int64_t(1) << 24) / (c.h_q * c.table_width);
+  return n < 1 ? 1 : (n < c.tokens ? n : c.tokens);
+}
+
+template <typename F>
+int with_dim(const moba_paged& c, F&& go) {
+  return MOBA_DISPATCH_DTYPE(static_cast<int>(c.dtype), T, [&] {
+    switch (c.head_dim) {
+      case 64: return go(T{}, std::integral_constant<int, 64>{});
+      case 128: return go(T{}, std::integral_constant<int, 128>{});
+      default: return go(T{}, std::integral_constant<int, 256>{});
+    }
+  });
+}
+
+int run_tiles(const moba_paged& c, GateArgs a, bool all_rows, hipStream_t s) {
+  const int64_t group = c.h_q / c.h_kv;
+  a.tile_tokens = static_cast<int>(128 / group);
+  const int64_t parts = cdiv(c.tokens, a.tile_tokens) + c.seqs;
+  return with_dim(c, [&](auto t, auto dim) {
+    using T = decltype(t);
+    constexpr int D = decltype(dim)::value;
+    if constexpr (sizeof(T) == 2) {
+      hipLaunchKernelGGL((norm_kernel<T, D / 16>), dim3(static_cast<unsigned>(c.seqs * c.h_kv), kNormParts),
+                         dim3(256), 0, s, a);
+      if (all_rows)
+        hipLaunchKernelGGL(nobody_kernel, dim3(static_cast<unsigned>(c.tokens)), dim3(64), 0, s, a);
+      auto go = [&](auto m, auto tm) {
+        hipLaunchKernelGGL((tiles_kernel<T, D, decltype(m)::value, decltype(tm)::value>),
+                           dim3(static_cast<unsigned>(parts), static_cast<unsigned>(c.h_kv)), dim3(256), 0, s, a);
+        return check_launch("moba_paged_gate (tiles)");
+      };
+      using std::integral_constant;
+      if (c.take <= 8) return go(integral_constant<int, 12>{}, integral_constant<int, 8>{});
+      if (c.take <= 16) return go(integral_constant<int, 20>{}, integral_constant<int, 16>{});
+      return go(integral_constant<int, 36>{}, integral_constant<int, 32>{});
+    } else {
+      return fail(MOBA_ERR_UNSUPPORTED, "unreachable");
+    }
+  });
+}
+
+}  // namespace
+
+size_t gate_workspace(const moba_paged& c) {
+  const size_t n = tiles_take(c) ? static_cast<size_t>(c.seqs * c.h_kv * kNormParts)
+                                 : static_cast<size_t>(score_slice(c) * c.h_q * c.table_width);
+  return (4 * n + 255) & ~size_t(255);
+}
+
+int gate_run(const moba_paged& c, const Paged& p, void* workspace, bool all_rows, hipStream_t s) {
+  GateArgs a;
+  a.p = p;
+  a.q = c.q;
+  a.kbar = c.kbar;
+  a.keys = a.norms = static_cast<uint32_t*>(workspace);
+  a.block_idx = c.block_idx;
+  a.h_q = static_cast<int>(c.h_q);
+  a.h_kv = static_cast<int>(c.h_kv);
+  a.slots = static_cast<int>(c.slots);
+  a.take = static_cast<int>(c.take);
+  a.current = c.always_current != 0;
+  if (tiles_take(c)) return run_tiles(c, a, all_rows, s);
+  const int64_t slice = score_slice(c);
+  for (int64_t t0 = 0; t0 < c.tokens; t0 += slice) {
+    a.tok0 = static_cast<int32_t>(t0);
+    a.slice = static_cast<int32_t>(c.tokens - t0 < slice ? c.tokens - t0 : slice);
+    int st = c.take == 0 ? MOBA_OK : with_dim(c, [&](auto t, auto dim) {
+      constexpr int LPR = decltype(dim)::value / 16;
+      const int64_t tiles = cdiv(c.table_width, kScoreThreads / LPR * kScoreRows);
+      if (tiles > 65535) return fail(MOBA_ERR_UNSUPPORTED, "block table too wide");
+      hipLaunchKernelGGL((score_kernel<decltype(t), LPR>),
+                         dim3(static_cast<unsigned>(a.slice * c.h_kv), static_cast<unsigned>(tiles)),
+                         dim3(kScoreThreads), 0, s, a);
+      return check_launch("moba_paged_gate (scores)");
+    });
+    if (st) return st;
+    const dim3 grid(static_cast<unsigned>(cdiv(a.slice * c.h_q, 4)));
+    if (c.take <= 8) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(256), 0, s, a);
+    else if (c.take <= 16) hipLaunchKernelGGL(select_kernel<16>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(select_kernel<32>, grid, dim3(256), 0, s, a);
+    st = check_launch("moba_paged_gate (select)");
+    if (st) return st;
+  }
+  return MOBA_OK;
+}
+
+}  // namespace moba
