@@ -403,7 +403,8 @@ int moba_append_tokens(const moba_paged* call, const void* k_new, const void* v_
  * over the blocks of block_idx (keys behind a token's own position stay
  * hidden; no visible key: out 0, lse -inf), moba_paged_attention does both.
  * moba_paged_layout sets workspace_bytes from the first group of fields.
- * take <= MOBA_PAGED_MAX_TAKE.
+ * take <= MOBA_PAGED_MAX_TAKE, table_width <= 65536. For
+ * moba_paged_attention block_idx may be NULL; otherwise it is scratch.
  */
 #define MOBA_PAGED_MAX_TAKE 32
 int moba_paged_layout(moba_paged* call);

@@ -30,41 +30,45 @@ struct NewTokens {
   int32_t first, n, len;
 };
 
+__device__ inline NewTokens checked_tokens(const Paged& p, int32_t first, int32_t end, int32_t len) {
+  const bool ok = first >= 0 && end > first && end <= p.tokens && len >= end - first;
+  return NewTokens{first, ok ? end - first : 0, len};
+}
+
 __device__ inline NewTokens new_tokens(const Paged& p, int32_t s) {
-  NewTokens r;
-  r.first = p.cu ? p.cu[s] : s * p.even;
-  const int32_t end = p.cu ? p.cu[s + 1] : r.first + p.even;
-  r.len = p.seq_lens[s];
-  const bool ok = r.first >= 0 && end > r.first && end <= p.tokens && r.len >= end - r.first;
-  r.n = ok ? end - r.first : 0;
-  return r;
+  const int32_t first = p.cu ? p.cu[s] : s * p.even;
+  return checked_tokens(p, first, p.cu ? p.cu[s + 1] : first + p.even, p.seq_lens[s]);
 }
 
 // Sequence and position of token `tok`, the same in all lanes of the wave;
 // position -1 where the token belongs to no sequence (rows behind the last
-// one, inconsistent lengths). Every lane compares one bound of 64, so up to
-// 64 sequences take one round of loads.
+// one, inconsistent lengths). Every lane holds the numbers of one of 64
+// sequences, so up to 64 sequences take one round of loads.
 struct TokenAt {
   int32_t seq, pos;
 };
 
-__device__ inline TokenAt locate(const Paged& p, int32_t tok) {
-  int32_t s = 0;
-  if (p.cu) {
-    const int lane = threadIdx.x & 63;
-    for (int32_t base = 0; base < p.seqs; base += 64) {
-      const int32_t i = base + lane;
-      s += __popcll(__ballot(i < p.seqs && p.cu[i < p.seqs ? i + 1 : p.seqs] <= tok));
-    }
-  } else {
-    s = tok / p.even;
-  }
-  TokenAt t{s, -1};
-  if (s >= p.seqs) return t;
-  const NewTokens r = new_tokens(p, s);
+__device__ inline TokenAt token_at(int32_t s, const NewTokens& r, int32_t tok) {
   const int32_t i = tok - r.first;
-  if (i >= 0 && i < r.n) t.pos = r.len - r.n + i;
-  return t;
+  return TokenAt{s, i >= 0 && i < r.n ? r.len - r.n + i : -1};
+}
+
+__device__ inline TokenAt locate(const Paged& p, int32_t tok) {
+  if (!p.cu) {
+    const int32_t s = tok / p.even;
+    return token_at(s, new_tokens(p, s), tok);
+  }
+  const int lane = threadIdx.x & 63;
+  for (int32_t base = 0; base < p.seqs; base += 64) {
+    const int32_t i = min(base + lane, p.seqs - 1);
+    const int32_t first = p.cu[i], end = p.cu[i + 1], len = p.seq_lens[i];
+    // Sequences up to the one that holds the token end at or before it.
+    const uint64_t behind = __ballot(base + lane < p.seqs && end > tok);
+    if (!behind) continue;
+    const int l = __builtin_ctzll(behind);
+    return token_at(base + l, checked_tokens(p, __shfl(first, l), __shfl(end, l), __shfl(len, l)), tok);
+  }
+  return TokenAt{0, -1};
 }
 
 // Page of block `blk` of sequence s, or -1 where the table has none.

@@ -16,30 +16,48 @@ struct RowArgs {
   const void* q;             // [tokens, h_q, D]
   const void* k;             // pages
   const void* v;
-  const int32_t* block_idx;  // [tokens, h_q, slots]
+  const int32_t* block_idx;  // [tokens, h_q, slots], or null: chosen here from
+  const uint32_t* keys;      // the scores [tokens, h_q, width]
   void* out;                 // [tokens, h_q, D]
   float* lse;                // [h_q, tokens] log2 units, or null
   float* part_ml;            // [rows, splits, 2]
   float* part_o;             // [rows, splits, D]
   int h_q, h_kv, slots, splits;
+  int take, current;
   float scale_log2;
 };
 
-constexpr int kRowWaves = 4;
+// A row's result from its maximum (log2 units), sum and weighted values. No
+// visible key: 0, lse -inf; a sum that is not a number stays one.
+__device__ inline float row_value(float x, float total) {
+  return total > 0.f ? x / total : (total == 0.f ? 0.f : x + total);
+}
+__device__ inline float row_lse(float top, float total) {
+  return total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
+}
 
 // One query head of one token per workgroup (and split): its chosen blocks in
 // runs of 64 / LPR * U keys, one run after another per wave. D / F lanes share
 // a key, F features each; every lane group keeps its own running maximum and
 // sum, and they meet at the end. All in float32.
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * kRowWaves) attend_rows_kernel(RowArgs a) {
+//
+// TM > 0: the blocks are chosen here, from the scores, by all waves: every
+// lane the best of every 64 NW-th score, every wave the best of its lanes, the
+// first wave the best of the waves (as select_kernel, without its launch and
+// its trip through memory).
+template <typename T, int D, int NW, int TM>
+__global__ void __launch_bounds__(64 * NW) attend_rows_kernel(RowArgs a) {
   constexpr int F = 16 / static_cast<int>(sizeof(T));
   constexpr int LPR = D / F;
   constexpr int RPW = 64 / LPR;  // keys per load instruction
   constexpr int U = 8;
   constexpr int KEYS = RPW * U;
-  __shared__ float s_o[kRowWaves][D];
-  __shared__ float s_m[kRowWaves], s_l[kRowWaves];
+  constexpr int TS = TM ? TM : 1;
+  using Best = WaveBest<Rank<T>, TS>;
+  __shared__ float s_o[NW][D];
+  __shared__ float s_m[NW], s_l[NW];
+  __shared__ typename Best::Word s_best[NW][TS];
+  __shared__ int32_t s_ids[TS + 1];
   const int64_t row = blockIdx.x;
   const int32_t tok = static_cast<int32_t>(row / a.h_q);
   const int h = static_cast<int>(row % a.h_q);
@@ -55,13 +73,33 @@ __global__ void __launch_bounds__(64 * kRowWaves) attend_rows_kernel(RowArgs a) 
 #pragma unroll
     for (int e = 0; e < F; ++e) q[e] = Elem<T>::load(qp, e) * a.scale_log2;
   }
+  const int32_t* ids = TM ? s_ids : a.block_idx + row * a.slots;
+  if constexpr (TM > 0) {
+    const int32_t own = at.pos / bs;
+    const int32_t past = a.take ? min(own, a.p.width) : 0;
+    Best list;
+    list.clear();
+    list.add_all(a.keys + row * a.p.width, past, wave * 64 + lane, 64 * NW);
+    list.meet();
+    if (lane < TM) s_best[wave][lane] = list.mine();
+    __syncthreads();
+    if (wave == 0) {
+      list.clear();
+#pragma unroll
+      for (int i = 0; i < NW * TM; i += 64)
+        if (i + lane < NW * TM) list.add((&s_best[0][0])[i + lane]);
+      list.meet();
+      list.emit(a.take, own_entry(a.p, a.current, at.seq, own), a.slots, s_ids);
+    }
+    __syncthreads();
+  }
   float m = -INFINITY, l = 0.f, o[F];
 #pragma unroll
   for (int e = 0; e < F; ++e) o[e] = 0.f;
   const int per_block = (bs + KEYS - 1) / KEYS;
   const int units = a.slots * per_block;
-  for (int u = blockIdx.y * kRowWaves + wave; u < units; u += a.splits * kRowWaves) {
-    const int32_t blk = a.block_idx[row * a.slots + u / per_block];
+  for (int u = blockIdx.y * NW + wave; u < units; u += a.splits * NW) {
+    const int32_t blk = ids[u / per_block];
     if (blk < 0) continue;
     const int32_t page = page_of(a.p, at.seq, blk);
     if (page < 0) continue;
@@ -134,17 +172,17 @@ __global__ void __launch_bounds__(64 * kRowWaves) attend_rows_kernel(RowArgs a) 
   __syncthreads();
   float top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, s_m[w]);
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, s_m[w]);
   const float z = top > -INFINITY ? top : 0.f;
   float total = 0.f;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) total += s_l[w] * __builtin_amdgcn_exp2f(s_m[w] - z);
-  for (int d = threadIdx.x; d < D; d += 64 * kRowWaves) {
+  for (int w = 0; w < NW; ++w) total += s_l[w] * __builtin_amdgcn_exp2f(s_m[w] - z);
+  for (int d = threadIdx.x; d < D; d += 64 * NW) {
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) x += s_o[w][d] * __builtin_amdgcn_exp2f(s_m[w] - z);
+    for (int w = 0; w < NW; ++w) x += s_o[w][d] * __builtin_amdgcn_exp2f(s_m[w] - z);
     if (a.splits == 1)
-      Elem<T>::store(static_cast<T*>(a.out) + row * D, d, total > 0.f ? x / total : (total == 0.f ? 0.f : x + total));
+      Elem<T>::store(static_cast<T*>(a.out) + row * D, d, row_value(x, total));
     else
       a.part_o[(row * a.splits + blockIdx.y) * D + d] = x;
   }
@@ -153,7 +191,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attend_rows_kernel(RowArgs a) 
       a.part_ml[(row * a.splits + blockIdx.y) * 2] = top;
       a.part_ml[(row * a.splits + blockIdx.y) * 2 + 1] = total;
     } else if (a.lse) {
-      a.lse[h * static_cast<int64_t>(a.p.tokens) + tok] = total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
+      a.lse[h * static_cast<int64_t>(a.p.tokens) + tok] = row_lse(top, total);
     }
   }
 }
@@ -181,15 +219,16 @@ __global__ void __launch_bounds__(64) merge_rows_kernel(RowArgs a) {
 #pragma unroll
   for (int e = 0; e < D / 64; ++e)
     Elem<T>::store(static_cast<T*>(a.out) + row * D, 64 * e + threadIdx.x,
-                   total > 0.f ? o[e] / total : (total == 0.f ? 0.f : o[e] + total));
+                   row_value(o[e], total));
   if (a.lse && threadIdx.x == 0)
-    a.lse[(row % a.h_q) * static_cast<int64_t>(a.p.tokens) + tok] = total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
+    a.lse[(row % a.h_q) * static_cast<int64_t>(a.p.tokens) + tok] = row_lse(top, total);
 }
 
 // How a call is cut up, and its workspace.
 struct PagedPlan {
+  int64_t waves;   // per workgroup of attend_rows_kernel
   int64_t splits;  // parts of a query's chosen blocks
-  size_t ml, o, total;
+  size_t ml, o, ids, total;
 };
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -197,20 +236,32 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // Keys per run of attend_rows_kernel.
 int64_t run_keys(int64_t D, int dtype) { return 64 * 8 / (D / (dtype == MOBA_FP32 ? 4 : 8)); }
 
+// Few queries: attend_rows_kernel chooses from the scores by itself.
+bool chooses_itself(const moba_paged& c) { return scores_only(c) && !chunk_takes(c); }
+
 PagedPlan plan_of(const moba_paged& c) {
   PagedPlan pl;
   const int64_t rows = c.tokens * c.h_q;
   const int64_t units = c.slots * cdiv(c.block_size, run_keys(c.head_dim, static_cast<int>(c.dtype)));
-  int64_t splits = cdiv(2048, rows * kRowWaves);
-  const int64_t most = cdiv(units, kRowWaves);
+  // Few rows: wide workgroups, and several of them per row.
+  pl.waves = rows < 256 && units > 4 ? 16 : 4;
+  const int64_t splits = cdiv(512, rows * pl.waves / 4);
+  const int64_t most = cdiv(units, pl.waves);
   pl.splits = splits < most ? splits : most;
   const size_t parts = pl.splits > 1 ? static_cast<size_t>(rows * pl.splits) : 0;
   pl.ml = align256(sizeof(float) * 2 * parts);
   pl.o = align256(sizeof(float) * c.head_dim * parts);
-  // The gate's scratch is free again when the attention starts.
-  const size_t attend = chunk_takes(c) ? chunk_plan(c).total : pl.ml + pl.o;
+  // The gate's scratch is free again when the blocks are chosen.
   const size_t gate = gate_workspace(c);
-  pl.total = attend > gate ? attend : gate;
+  if (chunk_takes(c)) {
+    const size_t attend = chunk_plan(c).total;
+    pl.total = attend > gate ? attend : gate;
+  } else {
+    pl.total = gate + pl.ml + pl.o;
+  }
+  // The chosen blocks, where the caller of moba_paged_attention has no use for them.
+  pl.ids = chooses_itself(c) ? 0 : align256(sizeof(int32_t) * static_cast<size_t>(rows * c.slots));
+  pl.total += pl.ids;
   return pl;
 }
 
@@ -219,6 +270,7 @@ int check_attention(const moba_paged* c, Paged* p) {
   if (st) return st;
   if (c->slots <= 0 || c->take < 0 || c->take + (c->always_current ? 1 : 0) > c->slots)
     return fail(MOBA_ERR_INVALID, "slots must hold the selected blocks");
+  if (c->table_width > 65536) return fail(MOBA_ERR_UNSUPPORTED, "more than 65536 blocks per sequence");
   if (c->take > MOBA_PAGED_MAX_TAKE)
     return fail(MOBA_ERR_UNSUPPORTED, "more than " + std::to_string(MOBA_PAGED_MAX_TAKE) +
                                           " past blocks per query");
@@ -291,52 +343,85 @@ static int run_gate(const moba_paged* c, bool all_rows, void* stream) {
 
 extern "C" int moba_paged_gate(const moba_paged* c, void* stream) { return run_gate(c, true, stream); }
 
-extern "C" int moba_paged_attend(const moba_paged* c, void* stream) {
+// `keys`: scores to choose from, or null where c.block_idx holds the blocks.
+static int run_attend(const moba_paged* c, const uint32_t* keys, void* stream) {
   using namespace moba;
   RowArgs a;
   int st = check_attention(c, &a.p);
   if (st) return st;
-  if (!aligned(c->q) || !aligned(c->k) || !aligned(c->v) || !aligned(c->out) || !c->block_idx)
+  if (!aligned(c->q) || !aligned(c->k) || !aligned(c->v) || !aligned(c->out) ||
+      !(keys || c->block_idx))
     return fail(MOBA_ERR_INVALID, "null or unaligned pointer");
   const PagedPlan pl = plan_of(*c);
   st = check_workspace(c, pl.total);
   if (st) return st;
+  hipStream_t s = as_stream(stream);
+  if (chunk_takes(*c)) return chunk_attend(*c, a.p, c->workspace, s);
+  char* scratch = static_cast<char*>(c->workspace) + gate_workspace(*c);
   a.q = c->q;
   a.k = c->k;
   a.v = c->v;
   a.block_idx = c->block_idx;
+  a.keys = keys;
   a.out = c->out;
   a.lse = c->lse;
-  a.part_ml = static_cast<float*>(c->workspace);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(c->workspace) + pl.ml);
+  a.part_ml = reinterpret_cast<float*>(scratch);
+  a.part_o = reinterpret_cast<float*>(scratch + pl.ml);
   a.h_q = static_cast<int>(c->h_q);
   a.h_kv = static_cast<int>(c->h_kv);
   a.slots = static_cast<int>(c->slots);
   a.splits = static_cast<int>(pl.splits);
+  a.take = static_cast<int>(c->take);
+  a.current = c->always_current != 0;
+  if (keys) a.slots = a.take + a.current;  // those it chooses; further ones are padding
   a.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(c->head_dim)));
-  hipStream_t s = as_stream(stream);
-  if (chunk_takes(*c)) return chunk_attend(*c, a.p, c->workspace, s);
   const int64_t rows = c->tokens * c->h_q;
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
-    auto go = [&](auto dim) {
-      constexpr int D = decltype(dim)::value;
-      hipLaunchKernelGGL((attend_rows_kernel<T, D>),
+    auto go = [&](auto dim, auto nw, auto tm) {
+      constexpr int D = decltype(dim)::value, NW = decltype(nw)::value, TM = decltype(tm)::value;
+      hipLaunchKernelGGL((attend_rows_kernel<T, D, NW, TM>),
                          dim3(static_cast<unsigned>(rows), static_cast<unsigned>(a.splits)),
-                         dim3(64 * kRowWaves), 0, s, a);
+                         dim3(64 * NW), 0, s, a);
       int rc = check_launch("moba_paged_attend");
       if (rc || a.splits == 1) return rc;
       hipLaunchKernelGGL((merge_rows_kernel<T, D>), dim3(static_cast<unsigned>(rows)), dim3(64), 0, s, a);
       return check_launch("moba_paged_attend (merge)");
     };
+    auto lists = [&](auto dim, auto nw) {
+      if (!keys) return go(dim, nw, std::integral_constant<int, 0>{});
+      if (a.take <= 8) return go(dim, nw, std::integral_constant<int, 8>{});
+      if (a.take <= 16) return go(dim, nw, std::integral_constant<int, 16>{});
+      return go(dim, nw, std::integral_constant<int, 32>{});
+    };
+    auto waves = [&](auto dim) {
+      if (pl.waves == 4) return lists(dim, std::integral_constant<int, 4>{});
+      return lists(dim, std::integral_constant<int, 16>{});
+    };
     switch (c->head_dim) {
-      case 64: return go(std::integral_constant<int, 64>{});
-      case 128: return go(std::integral_constant<int, 128>{});
-      default: return go(std::integral_constant<int, 256>{});
+      case 64: return waves(std::integral_constant<int, 64>{});
+      case 128: return waves(std::integral_constant<int, 128>{});
+      default: return waves(std::integral_constant<int, 256>{});
     }
   });
 }
 
+extern "C" int moba_paged_attend(const moba_paged* c, void* stream) { return run_attend(c, nullptr, stream); }
+
 extern "C" int moba_paged_attention(const moba_paged* c, void* stream) {
-  const int st = run_gate(c, false, stream);
-  return st ? st : moba_paged_attend(c, stream);
+  using namespace moba;
+  Paged p;
+  int st = check_attention(c, &p);
+  if (st) return st;
+  const PagedPlan pl = plan_of(*c);
+  if (chooses_itself(*c)) {
+    if (!aligned(c->q) || !aligned(c->kbar)) return fail(MOBA_ERR_INVALID, "null or unaligned pointer");
+    st = check_workspace(c, pl.total);
+    if (!st) st = gate_scores(*c, p, c->workspace, as_stream(stream));
+    return st ? st : run_attend(c, static_cast<const uint32_t*>(c->workspace), stream);
+  }
+  moba_paged call = *c;
+  if (!call.block_idx && call.workspace)
+    call.block_idx = reinterpret_cast<int32_t*>(static_cast<char*>(call.workspace) + pl.total - pl.ids);
+  st = run_gate(&call, false, stream);
+  return st ? st : run_attend(&call, nullptr, stream);
 }

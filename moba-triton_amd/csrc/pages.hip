@@ -16,7 +16,7 @@ struct AppendArgs {
   const void *wq, *wk;     // [D] or null
   const float *cosv, *sinv;
   int64_t table_len;
-  int h_q, h_kv, rotary, interleaved, w_f32;
+  int h_q, h_kv, rotary, w_f32;
   float eps;
 };
 
@@ -71,7 +71,7 @@ __device__ inline Piece find_piece(const Paged& p, int32_t piece) {
 constexpr int kAppendThreads = 256;
 constexpr int kQHeads = 4;
 
-template <typename T, int LPR>
+template <typename T, int LPR, bool IL>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
   constexpr int D = 16 * LPR;
   constexpr int G = kAppendThreads / LPR;  // lane groups: rows at a time
@@ -79,30 +79,40 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
   const Piece pc = find_piece(a.p, blockIdx.x);
   if (pc.seq < 0) return;
   const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR;
-  const RotLane rl = rot_lane(lane, a.rotary, a.interleaved);
+  const RotLane rl = rot_lane(lane, a.rotary, IL);
   const int n = pc.end - pc.begin;
   if (static_cast<int>(blockIdx.y) >= a.h_kv) {  // queries
     const int h0 = (static_cast<int>(blockIdx.y) - a.h_kv) * kQHeads;
     const int heads = a.h_q - h0 < kQHeads ? a.h_q - h0 : kQHeads;
     float w[16];
     if (a.wq) load16<T>(a.wq, a.w_f32, rl, w);
-    for (int i = g; i < n * heads; i += G) {
-      const int t = i / heads, h = h0 + i % heads;
-      const int64_t tok = pc.tok + t;
-      RawRow<T> raw;
-      raw.load(static_cast<const T*>(a.q) + tok * a.q_tok + h * a.q_head, rl);
-      float c[8], sn[8];
-      rot_turn(rl, a.cosv, a.sinv, a.rotary, pc.begin + t, a.table_len, c, sn);
-      float v[16];
-      raw.widen(v);
-      if (a.wq) {
-        const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
+    constexpr int R = 4;
+    for (int i0 = g; i0 < n * heads; i0 += R * G) {
+      RawRow<T> raw[R];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+      for (int u = 0; u < R; ++u) {
+        const int i = min(i0 + u * G, n * heads - 1);
+        raw[u].load(static_cast<const T*>(a.q) + static_cast<int64_t>(pc.tok + i / heads) * a.q_tok +
+                        (h0 + i % heads) * a.q_head, rl);
       }
-      rotate16(rl, c, sn, v);
-      raw.narrow(v);
-      raw.store(static_cast<T*>(a.q_out) + (tok * a.h_q + h) * D, rl);
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        const int last = n * heads - 1, i = min(i0 + u * G, last);
+        const int t = i / heads, h = h0 + i % heads;
+        float c[8], sn[8];
+        rot_turn(rl, a.cosv, a.sinv, a.rotary, pc.begin + t, a.table_len, c, sn);
+        float v[16];
+        raw[u].widen(v);
+        if (a.wq) {
+          const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+        }
+        rotate16<IL>(rl, c, sn, v);
+        raw[u].narrow(v);
+        if (i0 + u * G <= last)
+          raw[u].store(static_cast<T*>(a.q_out) + (static_cast<int64_t>(pc.tok + t) * a.h_q + h) * D, rl);
+      }
     }
     return;
   }
@@ -122,34 +132,50 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.0;
   if (full) {
-    for (int i = g; i < first; i += G) {
-      RawRow<T> raw;
-      raw.load(kp + static_cast<int64_t>(i) * D, rl);
+    constexpr int R = 4;
+    for (int i0 = g; i0 < first; i0 += R * G) {
+      RawRow<T> raw[R];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum[e] += static_cast<double>(raw.element(e));
+      for (int u = 0; u < R; ++u) raw[u].load(kp + static_cast<int64_t>(min(i0 + u * G, first - 1)) * D, rl);
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sum[e] += i0 + u * G < first ? static_cast<double>(raw[u].element(e)) : 0.0;
     }
   }
-  for (int i = g; i < n; i += G) {
-    const int64_t tok = pc.tok + i;
-    RawRow<T> raw, rv;
-    raw.load(static_cast<const T*>(a.k) + tok * a.k_tok + h * a.k_head, rl);
-    rv.load(static_cast<const T*>(a.v) + tok * a.v_tok + h * a.v_head, rl);
-    float c[8], sn[8];
-    rot_turn(rl, a.cosv, a.sinv, a.rotary, pc.begin + i, a.table_len, c, sn);
-    float v[16];
-    raw.widen(v);
-    if (a.wk) {
-      const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
+  constexpr int R = 2;
+  for (int i0 = g; i0 < n; i0 += R * G) {
+    RawRow<T> raw[R], rv[R];
+    float c[R][8], sn[R][8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+    for (int u = 0; u < R; ++u) {
+      const int i = min(i0 + u * G, n - 1);
+      const int64_t tok = pc.tok + i;
+      raw[u].load(static_cast<const T*>(a.k) + tok * a.k_tok + h * a.k_head, rl);
+      rv[u].load(static_cast<const T*>(a.v) + tok * a.v_tok + h * a.v_head, rl);
+      rot_turn(rl, a.cosv, a.sinv, a.rotary, pc.begin + i, a.table_len, c[u], sn[u]);
     }
-    rotate16(rl, c, sn, v);
-    raw.narrow(v);
-    raw.store(kp + static_cast<int64_t>(first + i) * D, rl);
-    rv.store(vp + static_cast<int64_t>(first + i) * D, rl);
-    if (full) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum[e] += static_cast<double>(raw.element(e));
+    for (int u = 0; u < R; ++u) {
+      const int i = i0 + u * G;
+      float v[16];
+      raw[u].widen(v);
+      if (a.wk) {
+        const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+      }
+      rotate16<IL>(rl, c[u], sn[u], v);
+      raw[u].narrow(v);
+      if (i < n) {
+        raw[u].store(kp + static_cast<int64_t>(first + i) * D, rl);
+        rv[u].store(vp + static_cast<int64_t>(first + i) * D, rl);
+        if (full) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum[e] += static_cast<double>(raw[u].element(e));
+        }
+      }
     }
   }
   if (!full) return;  // the same in the whole workgroup
@@ -260,7 +286,6 @@ extern "C" int moba_append_tokens(const moba_paged* c, const void* k_new, const 
   a.h_q = static_cast<int>(c->h_q);
   a.h_kv = static_cast<int>(c->h_kv);
   a.rotary = static_cast<int>(rotary);
-  a.interleaved = interleaved;
   a.w_f32 = weight_dtype == MOBA_FP32;
   a.eps = static_cast<float>(eps);
   // Runs of new tokens on one page: a sequence of n tokens has at most
@@ -270,10 +295,13 @@ extern "C" int moba_append_tokens(const moba_paged* c, const void* k_new, const 
             static_cast<unsigned>(a.h_kv + cdiv(a.h_q, kQHeads)));
   if (grid.y > 65535) return fail(MOBA_ERR_UNSUPPORTED, "append: too many heads");
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
-    auto go = [&](auto lpr) {
-      hipLaunchKernelGGL((append_kernel<T, decltype(lpr)::value>), grid, dim3(kAppendThreads), 0,
+    auto run = [&](auto lpr, auto il) {
+      hipLaunchKernelGGL((append_kernel<T, decltype(lpr)::value, decltype(il)::value>), grid, dim3(kAppendThreads), 0,
                          as_stream(stream), a);
       return check_launch("moba_append_tokens");
+    };
+    auto go = [&](auto lpr) {
+      return interleaved ? run(lpr, std::true_type{}) : run(lpr, std::false_type{});
     };
     switch (c->head_dim) {
       case 64: return go(std::integral_constant<int, 4>{});

@@ -13,8 +13,8 @@ namespace moba {
 // lanes behind the rotated part hold 16 consecutive features each.
 struct RotLane {
   int lo, hi;
-  int turn;  // 0: not rotated, 1: halves, 2: neighbours
-  int angle; // first of the lane's 8 angles
+  bool turn;       // rotated
+  int angle;       // first of the lane's 8 angles
 };
 
 __device__ inline RotLane rot_lane(int lane, int rotary, int interleaved) {
@@ -23,7 +23,7 @@ __device__ inline RotLane rot_lane(int lane, int rotary, int interleaved) {
   const bool halves = in && !interleaved;
   r.lo = halves ? 8 * lane : 16 * lane;
   r.hi = halves ? rotary / 2 + 8 * lane : 16 * lane + 8;
-  r.turn = in ? (interleaved ? 2 : 1) : 0;
+  r.turn = in;
   r.angle = 8 * lane;
   return r;
 }
@@ -51,32 +51,40 @@ __device__ inline void rot_turn(const RotLane& r, const float* cosv, const float
   }
 }
 
-// v[0, 8) are the features from lo, v[8, 16) those from hi.
+// v[0, 8) are the features from lo, v[8, 16) those from hi. By selects, not
+// branches: lanes that are not rotated keep their values whatever they are.
+// IL: neighbouring pairs (a template: a branch would let the compiler index
+// the row by it, in scratch memory).
+template <bool IL>
 __device__ inline void rotate16(const RotLane& r, const float (&c)[8], const float (&s)[8],
                                 float (&v)[16]) {
-  if (r.turn == 1) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = v[i], b = v[8 + i];
-      v[i] = a * c[i] - b * s[i];
-      v[8 + i] = b * c[i] + a * s[i];
-    }
-  } else if (r.turn == 2) {
+  const bool on = r.turn;
+  if constexpr (IL) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float a = v[2 * i], b = v[2 * i + 1];
-      v[2 * i] = a * c[i] - b * s[i];
-      v[2 * i + 1] = b * c[i] + a * s[i];
+      const float x = a * c[i] - b * s[i], y = b * c[i] + a * s[i];
+      v[2 * i] = on ? x : a;
+      v[2 * i + 1] = on ? y : b;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = v[i], b = v[8 + i];
+      const float x = a * c[i] - b * s[i], y = b * c[i] + a * s[i];
+      v[i] = on ? x : a;
+      v[8 + i] = on ? y : b;
     }
   }
 }
 
+template <bool IL>
 __device__ inline void unrotate16(const RotLane& r, const float (&c)[8], const float (&s)[8],
                                   float (&v)[16]) {
   float n[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) n[i] = -s[i];
-  rotate16(r, c, n, v);
+  rotate16<IL>(r, c, n, v);
 }
 
 __device__ inline float square_sum(const float (&v)[16]) {

@@ -37,9 +37,10 @@ struct RotSide {
   const void* w;      // [D], or null: no norm
   int64_t sb, ss, sh; // strides of x
   int heads;
-  int slices;         // lane groups that share a token's heads
+  int slices_log2;    // 2^ lane groups share a token's heads
   float* partial;     // backward: dw sums [workgroups, D]
   int blocks;         // workgroups of this side
+  int flat;           // the batch axis continues the token axis: sb = seq * ss
 };
 
 struct RotArgs {
@@ -47,8 +48,9 @@ struct RotArgs {
   const float* cosv;
   const float* sinv;
   const int32_t* positions;  // [batch * seq], or null: 0, 1, .. in each row
-  int64_t tokens, seq, table_len;
-  int rotary, interleaved, w_f32;
+  uint32_t tokens, seq;
+  int64_t table_len;
+  int rotary, w_f32;
   float eps;
 };
 
@@ -56,53 +58,70 @@ struct RotArgs {
 constexpr int kThreads = 256;
 constexpr int kRows = 4;
 
-template <typename T, int LPR>
+// Element offset of token `tok`'s first head.
+__device__ inline int64_t token_offset(const RotArgs& a, const RotSide& s, uint32_t tok) {
+  if (s.flat) return tok * s.ss;
+  const uint32_t b = tok / a.seq;
+  return b * s.sb + (tok - b * a.seq) * s.ss;
+}
+
+__device__ inline int32_t position_of(const RotArgs& a, uint32_t tok) {
+  if (a.positions) return a.positions[tok];
+  return static_cast<int32_t>(tok % a.seq);
+}
+
+// Workgroups stride over the side's lane groups' work, (token, slice of its
+// heads) pairs: one reading of the weights serves many rows.
+template <typename T, int LPR, bool IL>
 __global__ void __launch_bounds__(kThreads) norm_rotate_kernel(RotArgs a) {
   constexpr int D = 16 * LPR;
+  constexpr uint32_t kGroups = kThreads / LPR;
   const bool second = static_cast<int>(blockIdx.x) >= a.side[0].blocks;
   const RotSide s = a.side[second];
-  const int64_t block = static_cast<int64_t>(blockIdx.x) - (second ? a.side[0].blocks : 0);
+  const uint32_t block = blockIdx.x - (second ? a.side[0].blocks : 0);
   const int lane = threadIdx.x % LPR;
-  const int64_t group = (block * kThreads + threadIdx.x) / LPR;
-  const int64_t tok = group / s.slices;
-  if (tok >= a.tokens) return;  // whole lane groups
-  const int slice = static_cast<int>(group - tok * s.slices);
-  const RotLane rl = rot_lane(lane, a.rotary, a.interleaved);
-  float c[8], sn[8];
-  rot_turn(rl, a.cosv, a.sinv, a.rotary,
-           a.positions ? a.positions[tok] : static_cast<int32_t>(tok % a.seq), a.table_len, c, sn);
+  const RotLane rl = rot_lane(lane, a.rotary, IL);
   float w[16];
   if (s.w) load16<T>(s.w, a.w_f32, rl, w);
-  const T* x = static_cast<const T*>(s.x) + (tok / a.seq) * s.sb + (tok % a.seq) * s.ss;
-  T* y = static_cast<T*>(s.y) + tok * s.heads * D;
-  for (int h0 = slice; h0 < s.heads; h0 += kRows * s.slices) {
-    RawRow<T> raw[kRows];
+  const int slices = 1 << s.slices_log2;
+  const uint64_t work = static_cast<uint64_t>(a.tokens) << s.slices_log2;
+  for (uint64_t group = static_cast<uint64_t>(block) * kGroups + threadIdx.x / LPR; group < work;
+       group += static_cast<uint64_t>(s.blocks) * kGroups) {
+    const uint32_t tok = static_cast<uint32_t>(group >> s.slices_log2);
+    const int slice = static_cast<int>(group & (slices - 1));
+    if (slice >= s.heads) continue;
+    const T* x = static_cast<const T*>(s.x) + token_offset(a, s, tok);
+    T* y = static_cast<T*>(s.y) + static_cast<int64_t>(tok) * s.heads * D;
+    float c[8], sn[8];
+    rot_turn(rl, a.cosv, a.sinv, a.rotary, position_of(a, tok), a.table_len, c, sn);
+    for (int h0 = slice; h0 < s.heads; h0 += kRows << s.slices_log2) {
+      RawRow<T> raw[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int h = h0 + i * s.slices;
-      raw[i].load(x + static_cast<int64_t>(h < s.heads ? h : h0) * s.sh, rl);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int h = h0 + i * s.slices;
-      if (h >= s.heads) break;
-      float v[16];
-      raw[i].widen(v);
-      if (s.w) {
-        const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+      for (int i = 0; i < kRows; ++i) {
+        const int h = h0 + (i << s.slices_log2);
+        raw[i].load(x + (h < s.heads ? h : h0) * s.sh, rl);
       }
-      rotate16(rl, c, sn, v);
-      raw[i].narrow(v);
-      raw[i].store(y + static_cast<int64_t>(h) * D, rl);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int h = h0 + (i << s.slices_log2);
+        float v[16];
+        raw[i].widen(v);
+        if (s.w) {
+          const float r = rsqrtf(row_sum<LPR>(square_sum(v)) * (1.f / D) + a.eps);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
+        }
+        rotate16<IL>(rl, c, sn, v);
+        raw[i].narrow(v);
+        if (h < s.heads) raw[i].store(y + h * D, rl);
+      }
     }
   }
 }
 
 // dx, and this workgroup's share of dw. Workgroups of a side stride over its
 // lane groups' work, so the number of partial sums is bounded.
-template <typename T, int LPR>
+template <typename T, int LPR, bool IL>
 __global__ void __launch_bounds__(kThreads) norm_rotate_bwd_kernel(RotArgs a) {
   constexpr int D = 16 * LPR;
   constexpr int kGroups = kThreads / LPR;  // lane groups of the workgroup
@@ -112,37 +131,39 @@ __global__ void __launch_bounds__(kThreads) norm_rotate_bwd_kernel(RotArgs a) {
   const RotSide s = a.side[second];
   const int64_t block = static_cast<int64_t>(blockIdx.x) - (second ? a.side[0].blocks : 0);
   const int lane = threadIdx.x % LPR;
-  const RotLane rl = rot_lane(lane, a.rotary, a.interleaved);
+  const RotLane rl = rot_lane(lane, a.rotary, IL);
   float w[16], dw[16];
   if (s.w) load16<T>(s.w, a.w_f32, rl, w);
 #pragma unroll
   for (int e = 0; e < 16; ++e) dw[e] = 0.f;
-  const int64_t work = a.tokens * s.slices;
-  for (int64_t group = block * kGroups + threadIdx.x / LPR; group < work;
-       group += static_cast<int64_t>(s.blocks) * kGroups) {
-    const int64_t tok = group / s.slices;
-    const int slice = static_cast<int>(group - tok * s.slices);
+  const int slices = 1 << s.slices_log2;
+  const uint64_t work = static_cast<uint64_t>(a.tokens) << s.slices_log2;
+  for (uint64_t group = static_cast<uint64_t>(block) * kGroups + threadIdx.x / LPR; group < work;
+       group += static_cast<uint64_t>(s.blocks) * kGroups) {
+    const uint32_t tok = static_cast<uint32_t>(group >> s.slices_log2);
+    const int slice = static_cast<int>(group & (slices - 1));
+    if (slice >= s.heads) continue;
+    const T* x = static_cast<const T*>(s.x) + token_offset(a, s, tok);
+    const T* dy = static_cast<const T*>(s.dy) + static_cast<int64_t>(tok) * s.heads * D;
+    T* dx = static_cast<T*>(s.y) + static_cast<int64_t>(tok) * s.heads * D;
     float c[8], sn[8];
-    rot_turn(rl, a.cosv, a.sinv, a.rotary,
-             a.positions ? a.positions[tok] : static_cast<int32_t>(tok % a.seq), a.table_len, c, sn);
-    const T* x = static_cast<const T*>(s.x) + (tok / a.seq) * s.sb + (tok % a.seq) * s.ss;
-    const T* dy = static_cast<const T*>(s.dy) + tok * s.heads * D;
-    T* dx = static_cast<T*>(s.y) + tok * s.heads * D;
-    for (int h0 = slice; h0 < s.heads; h0 += R * s.slices) {
+    rot_turn(rl, a.cosv, a.sinv, a.rotary, position_of(a, tok), a.table_len, c, sn);
+    for (int h0 = slice; h0 < s.heads; h0 += R << s.slices_log2) {
       RawRow<T> rx[R], rg[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const int h = h0 + i * s.slices < s.heads ? h0 + i * s.slices : h0;
-        rg[i].load(dy + static_cast<int64_t>(h) * D, rl);
-        if (s.w) rx[i].load(x + static_cast<int64_t>(h) * s.sh, rl);
+        const int hi = h0 + (i << s.slices_log2);
+        const int h = hi < s.heads ? hi : h0;
+        rg[i].load(dy + h * D, rl);
+        if (s.w) rx[i].load(x + h * s.sh, rl);
       }
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const int h = h0 + i * s.slices;
-        if (h >= s.heads) break;
+        const int h = h0 + (i << s.slices_log2);
+        const bool in = h < s.heads;  // a row past the last counts nowhere
         float g[16];
         rg[i].widen(g);
-        unrotate16(rl, c, sn, g);
+        unrotate16<IL>(rl, c, sn, g);
         if (s.w) {
           float v[16];
           rx[i].widen(v);
@@ -151,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) norm_rotate_bwd_kernel(RotArgs a) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             v[e] *= r;
-            dw[e] = fmaf(g[e], v[e], dw[e]);
+            dw[e] = in ? fmaf(g[e], v[e], dw[e]) : dw[e];
             g[e] *= w[e];
             dot = fmaf(g[e], v[e], dot);
           }
@@ -160,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) norm_rotate_bwd_kernel(RotArgs a) {
           for (int e = 0; e < 16; ++e) g[e] = r * (g[e] - v[e] * dot);
         }
         rg[i].narrow(g);
-        rg[i].store(dx + static_cast<int64_t>(h) * D, rl);
+        if (in) rg[i].store(dx + h * D, rl);
       }
     }
   }
@@ -188,28 +209,31 @@ __global__ void __launch_bounds__(kThreads) norm_rotate_bwd_kernel(RotArgs a) {
 }
 
 // dw[d] = sum over the workgroups' partial sums, float64, in a fixed order:
-// 16 threads per feature take every 16th workgroup and meet by shuffles.
+// 64 threads per feature take every 64th workgroup and meet in LDS (16
+// threads per feature: 15 us for 1638 workgroups of 128 features, 64: 7).
 // grid (D / 16, 2).
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 norm_weight_kernel(const float* __restrict__ pq, int nq, W* __restrict__ dwq,
                    const float* __restrict__ pk, int nk, W* __restrict__ dwk, int D) {
   const float* p = blockIdx.y ? pk : pq;
   const int n = blockIdx.y ? nk : nq;
   W* out = blockIdx.y ? dwk : dwq;
   if (!out) return;
-  // Lanes along the features (64-byte reads), partial sums through LDS.
-  __shared__ double part[16][17];
+  // Lanes along the features: 64-byte reads.
+  __shared__ double part[64][17];
   const int d = threadIdx.x & 15, j = threadIdx.x >> 4;
   const int feature = blockIdx.x * 16 + d;
   double t = 0.0;
-#pragma unroll 4
-  for (int i = j; i < n; i += 16) t += static_cast<double>(p[static_cast<int64_t>(i) * D + feature]);
+#pragma unroll 8
+  for (int i = j; i < n; i += 64) t += static_cast<double>(p[static_cast<int64_t>(i) * D + feature]);
   part[j][d] = t;
   __syncthreads();
-  if (j) return;
-  for (int i = 1; i < 16; ++i) t += part[i][d];
-  Elem<W>::store(out, feature, static_cast<float>(t));
+  if (j >= 4) return;
+  for (int i = j + 4; i < 64; i += 4) t += part[i][d];
+  t += __shfl_xor(t, 16);
+  t += __shfl_xor(t, 32);
+  if (j == 0) Elem<W>::store(out, feature, static_cast<float>(t));
 }
 
 int check(int64_t batch, int64_t seq, int64_t h_q, int64_t h_kv, int64_t D, int64_t rotary,
@@ -218,8 +242,9 @@ int check(int64_t batch, int64_t seq, int64_t h_q, int64_t h_kv, int64_t D, int6
     return fail(MOBA_ERR_INVALID, "non-positive shape argument");
   const int st = check_rotary(D, rotary, table_len, cosv, sinv, dtype, w_dtype);
   if (st) return st;
-  if (batch * seq > (int64_t(1) << 31) - 1)
+  if (batch > INT32_MAX / seq)
     return fail(MOBA_ERR_UNSUPPORTED, "norm_rotate: more than 2^31 - 1 tokens");
+  if (h_q > 65536 || h_kv > 65536) return fail(MOBA_ERR_UNSUPPORTED, "norm_rotate: too many heads");
   return MOBA_OK;
 }
 
@@ -236,51 +261,68 @@ int check_rows(std::initializer_list<const void*> rows, const int64_t* strides, 
   return MOBA_OK;
 }
 
-// Lane groups per token: one group holds kRows heads at a time; a call with
-// few rows takes a group for each head instead, so the rows are in flight at
-// once on an otherwise idle chip.
-int slices_of(int64_t tokens, int heads) {
-  const int few = (heads + kRows - 1) / kRows;
-  return tokens * heads <= 1 << 15 ? heads : few;
+// log2 of the lane groups per token: a group holds kRows heads at a time; a
+// call with few rows takes a group for each head instead, so the rows are in
+// flight at once on an otherwise idle chip.
+int slices_log2(int64_t tokens, int64_t heads) {
+  const int64_t want = tokens * heads <= 1 << 15 ? heads : heads / kRows;
+  int n = 0;
+  while ((int64_t(2) << n) <= want) ++n;
+  if (tokens * heads <= 1 << 15 && (int64_t(1) << n) < heads) ++n;
+  return n;
 }
 
 template <typename F>
-int with_lanes(int64_t D, F&& go) {
+int with_lanes(int64_t D, int interleaved, F&& go) {
+  auto pairs = [&](auto lpr) {
+    return interleaved ? go(lpr, std::true_type{}) : go(lpr, std::false_type{});
+  };
   switch (D) {
-    case 32: return go(std::integral_constant<int, 2>{});
-    case 64: return go(std::integral_constant<int, 4>{});
-    case 128: return go(std::integral_constant<int, 8>{});
-    case 256: return go(std::integral_constant<int, 16>{});
-    case 512: return go(std::integral_constant<int, 32>{});
-    default: return go(std::integral_constant<int, 64>{});
+    case 32: return pairs(std::integral_constant<int, 2>{});
+    case 64: return pairs(std::integral_constant<int, 4>{});
+    case 128: return pairs(std::integral_constant<int, 8>{});
+    case 256: return pairs(std::integral_constant<int, 16>{});
+    case 512: return pairs(std::integral_constant<int, 32>{});
+    default: return pairs(std::integral_constant<int, 64>{});
   }
 }
 
-// Workgroups of one side of the backward: at most kBwdBlocks in all, so that
-// a lane sums tens of rows before it meets the others.
-constexpr int64_t kBwdBlocks = 2048;
-int64_t bwd_blocks(int64_t tokens, int slices, int64_t D, int64_t share) {
-  const int64_t need = cdiv(tokens * slices, kThreads / (D / 16));
-  return need < share ? need : share;
+// Workgroups of a call, at most kMaxBlocks, shared by the sides' rows.
+constexpr int64_t kMaxBlocks = 2048;
+void set_blocks(RotArgs* a, int64_t head_dim) {
+  const int64_t h_q = a->side[0].heads, h_kv = a->side[1].heads;
+  int64_t share = kMaxBlocks * h_q / (h_q + h_kv);
+  share = share < 1 ? 1 : (share < kMaxBlocks ? share : kMaxBlocks - 1);
+  for (int i = 0; i < 2; ++i) {
+    RotSide& s = a->side[i];
+    const int64_t need = cdiv(static_cast<int64_t>(a->tokens) << s.slices_log2, kThreads / (head_dim / 16));
+    const int64_t most = i ? kMaxBlocks - share : share;
+    s.blocks = static_cast<int>(need < most ? need : most);
+  }
 }
 
 RotArgs make_args(const void* q, const void* k, void* yq, void* yk, const float* cosv,
                   const float* sinv, const int32_t* positions, const void* wq, const void* wk,
                   int64_t batch, int64_t seq, int64_t h_q, int64_t h_kv, const int64_t* strides,
-                  int64_t rotary, int64_t table_len, int interleaved, double eps, int w_dtype) {
+                  int64_t rotary, int64_t table_len, double eps, int w_dtype) {
   RotArgs a;
-  a.side[0] = {q, nullptr, yq, wq, strides[0], strides[1], strides[2], static_cast<int>(h_q),
-               slices_of(batch * seq, static_cast<int>(h_q)), nullptr, 0};
-  a.side[1] = {k, nullptr, yk, wk, strides[3], strides[4], strides[5], static_cast<int>(h_kv),
-               slices_of(batch * seq, static_cast<int>(h_kv)), nullptr, 0};
+  const void* x[2] = {q, k};
+  void* y[2] = {yq, yk};
+  const void* w[2] = {wq, wk};
+  const int64_t heads[2] = {h_q, h_kv};
+  for (int i = 0; i < 2; ++i) {
+    RotSide& s = a.side[i];
+    s = RotSide{x[i], nullptr, y[i], w[i], strides[3 * i], strides[3 * i + 1], strides[3 * i + 2],
+                static_cast<int>(heads[i]), slices_log2(batch * seq, heads[i]), nullptr, 0, 0};
+    s.flat = batch == 1 || s.sb == seq * s.ss;
+  }
   a.cosv = cosv;
   a.sinv = sinv;
   a.positions = positions;
-  a.tokens = batch * seq;
-  a.seq = seq;
+  a.tokens = static_cast<uint32_t>(batch * seq);
+  a.seq = static_cast<uint32_t>(seq);
   a.table_len = table_len;
   a.rotary = static_cast<int>(rotary);
-  a.interleaved = interleaved;
   a.w_f32 = w_dtype == MOBA_FP32;
   a.eps = static_cast<float>(eps);
   return a;
@@ -318,16 +360,12 @@ extern "C" int moba_norm_rotate(const void* q, const void* k, void* q_out, void*
   if (!st) st = check_rows({q, k, q_out, k_out}, strides, dtype);
   if (st) return st;
   RotArgs a = make_args(q, k, q_out, k_out, cos_table, sin_table, positions, q_weight, k_weight,
-                        batch, seq_len, h_q, h_kv, strides, rotary, table_len, interleaved, eps,
+                        batch, seq_len, h_q, h_kv, strides, rotary, table_len, eps,
                         weight_dtype);
-  for (RotSide& s : a.side) {
-    const int64_t blocks = cdiv(a.tokens * s.slices, kThreads / (head_dim / 16));
-    if (blocks > (1 << 30)) return fail(MOBA_ERR_UNSUPPORTED, "norm_rotate: too many rows");
-    s.blocks = static_cast<int>(blocks);
-  }
+  set_blocks(&a, head_dim);
   return MOBA_DISPATCH_DTYPE(dtype, T, [&] {
-    return with_lanes(head_dim, [&](auto lpr) {
-      hipLaunchKernelGGL((norm_rotate_kernel<T, decltype(lpr)::value>),
+    return with_lanes(head_dim, interleaved, [&](auto lpr, auto il) {
+      hipLaunchKernelGGL((norm_rotate_kernel<T, decltype(lpr)::value, decltype(il)::value>),
                          dim3(static_cast<unsigned>(a.side[0].blocks + a.side[1].blocks)),
                          dim3(kThreads), 0, as_stream(stream), a);
       return check_launch("moba_norm_rotate");
@@ -336,7 +374,7 @@ extern "C" int moba_norm_rotate(const void* q, const void* k, void* q_out, void*
 }
 
 extern "C" size_t moba_norm_rotate_bwd_workspace_size(int64_t head_dim) {
-  return sizeof(float) * static_cast<size_t>(moba::kBwdBlocks * (head_dim > 0 ? head_dim : 0));
+  return sizeof(float) * static_cast<size_t>(moba::kMaxBlocks * (head_dim > 0 ? head_dim : 0));
 }
 
 extern "C" int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, const void* q,
@@ -357,16 +395,11 @@ extern "C" int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, cons
       (k_weight != nullptr) != (dk_weight != nullptr))
     return fail(MOBA_ERR_INVALID, "a norm weight and its gradient go together");
   RotArgs a = make_args(q, k, dq, dk, cos_table, sin_table, positions, q_weight, k_weight, batch,
-                        seq_len, h_q, h_kv, strides, rotary, table_len, interleaved, eps,
+                        seq_len, h_q, h_kv, strides, rotary, table_len, eps,
                         weight_dtype);
   a.side[0].dy = dq_out;
   a.side[1].dy = dk_out;
-  // Each side's share of the workgroups goes by its rows.
-  int64_t share = kBwdBlocks * h_q / (h_q + h_kv);
-  share = share < 1 ? 1 : (share < kBwdBlocks ? share : kBwdBlocks - 1);
-  a.side[0].blocks = static_cast<int>(bwd_blocks(a.tokens, a.side[0].slices, head_dim, share));
-  a.side[1].blocks =
-      static_cast<int>(bwd_blocks(a.tokens, a.side[1].slices, head_dim, kBwdBlocks - share));
+  set_blocks(&a, head_dim);
   if (q_weight || k_weight) {
     if (!workspace || workspace_bytes < moba_norm_rotate_bwd_workspace_size(head_dim))
       return fail(MOBA_ERR_WORKSPACE, "norm_rotate_bwd workspace too small");
@@ -374,8 +407,8 @@ extern "C" int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, cons
     a.side[1].partial = a.side[0].partial + a.side[0].blocks * head_dim;
   }
   st = MOBA_DISPATCH_DTYPE(dtype, T, [&] {
-    return with_lanes(head_dim, [&](auto lpr) {
-      hipLaunchKernelGGL((norm_rotate_bwd_kernel<T, decltype(lpr)::value>),
+    return with_lanes(head_dim, interleaved, [&](auto lpr, auto il) {
+      hipLaunchKernelGGL((norm_rotate_bwd_kernel<T, decltype(lpr)::value, decltype(il)::value>),
                          dim3(static_cast<unsigned>(a.side[0].blocks + a.side[1].blocks)),
                          dim3(kThreads), 0, as_stream(stream), a);
       return check_launch("moba_norm_rotate_bwd");
@@ -384,7 +417,7 @@ extern "C" int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, cons
   if (st || !(q_weight || k_weight)) return st;
   return MOBA_DISPATCH_DTYPE(weight_dtype, W, [&] {
     hipLaunchKernelGGL(norm_weight_kernel<W>, dim3(static_cast<unsigned>(head_dim / 16), 2),
-                       dim3(256), 0, as_stream(stream), a.side[0].partial, a.side[0].blocks,
+                       dim3(1024), 0, as_stream(stream), a.side[0].partial, a.side[0].blocks,
                        static_cast<W*>(dq_weight), a.side[1].partial, a.side[1].blocks,
                        static_cast<W*>(dk_weight), static_cast<int>(head_dim));
     return check_launch("moba_norm_rotate_bwd (weights)");

@@ -131,22 +131,19 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-class on_device:
-    """Launches inside go to `device`, whichever is the current one."""
+def addr(t: torch.Tensor | None) -> int | None:
+    """Device address of a tensor as a number (None -> NULL)."""
+    return None if t is None else t.data_ptr()
 
-    def __init__(self, device: torch.device):
-        index = device.index
-        self._guard = None
-        if index is not None and index != torch.cuda.current_device():
-            self._guard = torch.cuda.device(index)
 
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def call_on(device: torch.device, name: str, *args) -> None:
+    """`call` with the current stream of `device` as the last argument,
+    launching there whichever device is the current one."""
+    if device.index == torch._C._cuda_getDevice():
+        call(name, *args, raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, raw_stream(device))
 
 
 def available() -> tuple[bool, str]:
@@ -168,6 +165,12 @@ def ptr(t: torch.Tensor | None):
 def stream_handle(device: torch.device):
     """The current torch stream on `device`, as a hipStream_t."""
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device: torch.device) -> int:
+    """As `stream_handle`, an address without the objects around it: a short
+    call's host work is most of its time (0.2 us against 3)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def call(name: str, *args) -> None:
@@ -204,7 +207,7 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(
                 f"moba HIP kernels need GPU tensors, got a tensor on {t.device}")
         if dev is None:
@@ -220,9 +223,13 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` itself where its rows (the last axis) can be read in 16-byte pieces
     at its strides, else a contiguous copy."""
     piece = 16 // t.element_size()
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and \
-            all(s % piece == 0 for s in t.stride()[:-1]):
-        return t
+    *outer, last = t.stride()
+    if last == 1 and t.data_ptr() % 16 == 0:
+        for s in outer:
+            if s % piece:
+                break
+        else:
+            return t
     return aligned_contiguous(t)
 
 

@@ -25,6 +25,8 @@ from moba.kernels.rotary import check_tables, check_weights
 HEAD_DIMS = (64, 128, 256)
 MAX_BLOCK = 1024
 MAX_TAKE = 32  # past blocks per query
+MAX_BLOCKS = 1 << 16  # per sequence
+_Strides = ctypes.c_int64 * 6
 
 
 @dataclass(frozen=True)
@@ -42,22 +44,23 @@ class PagedKV:
 
     def __post_init__(self) -> None:
         k, v, kbar = self.k, self.v, self.kbar
-        if k.ndim not in (4, 5) or k.shape != v.shape:
+        shape = k.shape
+        if len(shape) not in (4, 5) or v.shape != shape:
             raise ValueError(f"pages must be [(layers,) pages, H_kv, block, D], got "
-                             f"{tuple(k.shape)}, {tuple(v.shape)}")
-        if kbar.shape != k.shape[:-2] + k.shape[-1:]:
+                             f"{tuple(shape)}, {tuple(v.shape)}")
+        if kbar.shape != shape[:-2] + shape[-1:]:
             raise ValueError(f"kbar shape {tuple(kbar.shape)} does not match pages "
-                             f"{tuple(k.shape)}")
-        if not (k.dtype == v.dtype == kbar.dtype):
+                             f"{tuple(shape)}")
+        if k.dtype is not v.dtype or k.dtype is not kbar.dtype:
             raise ValueError(f"dtype mismatch: {k.dtype}, {v.dtype}, {kbar.dtype}")
         if k.dtype not in _lib.DTYPE_CODE:
             raise ValueError(f"unsupported dtype {k.dtype}")
-        if 0 in k.shape:
-            raise ValueError(f"empty cache: {tuple(k.shape)}")
-        if k.shape[-1] not in HEAD_DIMS:
-            raise ValueError(f"paged caches take head_dim {HEAD_DIMS}, got {k.shape[-1]}")
-        if not TENSOR_CORE_TILE <= k.shape[-2] <= MAX_BLOCK:
-            raise ValueError(f"block_size {k.shape[-2]} must be from {TENSOR_CORE_TILE} to "
+        if 0 in shape:
+            raise ValueError(f"empty cache: {tuple(shape)}")
+        if shape[-1] not in HEAD_DIMS:
+            raise ValueError(f"paged caches take head_dim {HEAD_DIMS}, got {shape[-1]}")
+        if not TENSOR_CORE_TILE <= shape[-2] <= MAX_BLOCK:
+            raise ValueError(f"block_size {shape[-2]} must be from {TENSOR_CORE_TILE} to "
                              f"{MAX_BLOCK}")
         for t in (k, v, kbar):
             if not t.is_contiguous() or t.data_ptr() % 16:
@@ -82,40 +85,42 @@ class PagedKV:
 def _call(q, cache: PagedKV, block_table, seq_lens, cu_seqlens) -> _lib.Paged:
     """The checked call on one layer's pages, without its stage's pointers
     (the device is the caller's to check)."""
-    if cache.k.ndim != 4:
+    shape, qs = cache.k.shape, q.shape
+    if len(shape) != 4:
         raise ValueError("one layer's pages are needed: use PagedKV.layer")
-    pages, h_kv, block, d = cache.k.shape
-    if q.ndim != 3 or q.shape[2] != d:
-        raise ValueError(f"queries must be [tokens, H_q, {d}], got {tuple(q.shape)}")
-    if q.dtype != cache.k.dtype:
+    pages, h_kv, block, d = shape
+    if len(qs) != 3 or qs[2] != d:
+        raise ValueError(f"queries must be [tokens, H_q, {d}], got {tuple(qs)}")
+    if q.dtype is not cache.k.dtype:
         raise ValueError(f"dtype mismatch: {q.dtype}, cache {cache.k.dtype}")
-    head_group_size(q.shape[1], h_kv)
-    if block_table.ndim != 2 or seq_lens.ndim != 1 or 0 in block_table.shape or \
-            seq_lens.shape[0] != block_table.shape[0]:
+    tokens, h_q, _ = qs
+    head_group_size(h_q, h_kv)
+    ts, ls = block_table.shape, seq_lens.shape
+    if len(ts) != 2 or len(ls) != 1 or 0 in ts or ls[0] != ts[0]:
         raise ValueError(f"block_table must be [sequences, blocks] and seq_lens [sequences], got "
-                         f"{tuple(block_table.shape)}, {tuple(seq_lens.shape)}")
-    seqs, width = block_table.shape
+                         f"{tuple(ts)}, {tuple(ls)}")
+    seqs, width = ts
     for name, t in (("block_table", block_table), ("seq_lens", seq_lens), ("cu_seqlens", cu_seqlens)):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous int32")
     if cu_seqlens is None:
-        if q.shape[0] % seqs:
-            raise ValueError(f"{q.shape[0]} tokens do not divide over {seqs} sequences: "
+        if tokens % seqs:
+            raise ValueError(f"{tokens} tokens do not divide over {seqs} sequences: "
                              "cu_seqlens is needed")
-    elif tuple(cu_seqlens.shape) != (seqs + 1,):
+        even, cu = tokens // seqs, None
+    elif cu_seqlens.shape != (seqs + 1,):
         raise ValueError(f"cu_seqlens must be [{seqs + 1}], got {tuple(cu_seqlens.shape)}")
-    call = _lib.Paged(q.shape[0], seqs, q.shape[1], h_kv, d, block, width, pages,
-                      _lib.DTYPE_CODE[q.dtype], q.shape[0] // seqs if cu_seqlens is None else 0)
-    call.k, call.v, call.kbar = cache.k.data_ptr(), cache.v.data_ptr(), cache.kbar.data_ptr()
-    call.block_table, call.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
-    call.cu_seqlens = None if cu_seqlens is None else cu_seqlens.data_ptr()
-    return call
+    else:
+        even, cu = 0, cu_seqlens.data_ptr()
+    return _lib.Paged(tokens, seqs, h_q, h_kv, d, block, width, pages, _lib.DTYPE_CODE[q.dtype],
+                      even, 0, 0, 0, 0, None, cache.k.data_ptr(), cache.v.data_ptr(),
+                      cache.kbar.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu)
 
 
 def _output(out, q):
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+    if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
     if not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be contiguous and 16-byte aligned")
@@ -155,10 +160,10 @@ def append_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
         ValueError: On mismatched shapes, dtypes, tables or weights.
     """
     if k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or \
-            k.shape[1:] != (cache.k.shape[-3], cache.k.shape[-1]):
+            k.shape[1] != cache.k.shape[-3] or k.shape[2] != cache.k.shape[-1]:
         raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v "
                          f"{tuple(v.shape)}, pages {tuple(cache.k.shape)}")
-    if not (q.dtype == k.dtype == v.dtype):
+    if q.dtype is not k.dtype or q.dtype is not v.dtype:
         raise ValueError(f"dtype mismatch: {q.dtype}, {k.dtype}, {v.dtype}")
     call = _call(q, cache, block_table, seq_lens, cu_seqlens)
     code = check_weights(q, q_weight, k_weight)
@@ -168,16 +173,21 @@ def append_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     out = _output(out, q)
     if q.shape[0] == 0:
         return out
-    q, k, v = (_lib.aligned_rows(t) for t in (q, k, v))
-    cos, sin, q_weight, k_weight = (None if t is None else _lib.aligned_contiguous(t)
-                                    for t in (cos, sin, q_weight, k_weight))
+    q, k, v = _lib.aligned_rows(q), _lib.aligned_rows(k), _lib.aligned_rows(v)
+    length = 0
+    if rotary:
+        cos, sin = _lib.aligned_contiguous(cos), _lib.aligned_contiguous(sin)
+        length = cos.shape[0]
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
     call.q = q.data_ptr()
-    strides = (ctypes.c_int64 * 6)(*(s for t in (q, k, v) for s in t.stride()[:2]))
-    with _lib.on_device(dev):
-        _lib.call("moba_append_tokens", ctypes.byref(call), _lib.ptr(k), _lib.ptr(v), strides,
-                  *map(_lib.ptr, (out, cos, sin, q_weight, k_weight)), rotary,
-                  0 if cos is None else cos.shape[0], int(bool(interleaved)), float(eps), code,
-                  _lib.stream_handle(dev))
+    strides = _Strides(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    a = _lib.addr
+    _lib.call_on(dev, "moba_append_tokens", ctypes.byref(call), k.data_ptr(), v.data_ptr(), strides,
+                 out.data_ptr(), a(cos), a(sin), a(q_weight), a(k_weight), rotary, length,
+                 bool(interleaved), float(eps), code)
     return out
 
 
@@ -188,6 +198,8 @@ def _attention_call(q, cache, block_table, seq_lens, cu_seqlens, cfg: MoBAConfig
                          f"{cache.k.shape[2]}")
     if cfg.gate_group > 0:
         raise ValueError("the hierarchical gate (gate_group > 0) takes no paged cache")
+    if call.table_width > MAX_BLOCKS:
+        raise ValueError(f"block_table has {call.table_width} blocks per sequence, at most {MAX_BLOCKS}")
     call.take = cfg.past_blocks_selected(call.table_width)
     if call.take > MAX_TAKE:
         raise ValueError(f"top_k {cfg.top_k}: at most {MAX_TAKE} past blocks per query")
@@ -200,14 +212,13 @@ def _attention_call(q, cache, block_table, seq_lens, cu_seqlens, cfg: MoBAConfig
 def _run(name, dev, call, q, block_idx, out, lse):
     q = _lib.aligned_contiguous(q)
     call.q = q.data_ptr()
-    call.block_idx = block_idx.data_ptr()
+    call.block_idx = None if block_idx is None else block_idx.data_ptr()
     call.out = None if out is None else out.data_ptr()
     call.lse = None if lse is None else lse.data_ptr()
     _lib.call("moba_paged_layout", ctypes.byref(call))
     workspace = torch.empty(call.workspace_bytes, device=dev, dtype=torch.uint8)
     call.workspace = workspace.data_ptr()
-    with _lib.on_device(dev):
-        _lib.call(name, ctypes.byref(call), _lib.stream_handle(dev))
+    _lib.call_on(dev, name, ctypes.byref(call))
 
 
 def paged_gate_select(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor,
@@ -270,9 +281,6 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor,
         call.slots, call.take = block_idx.shape[2], 0
         name = "moba_paged_attend"
     if q.shape[0]:
-        if block_idx is None:
-            block_idx = torch.empty((q.shape[0], q.shape[1], call.slots), dtype=torch.int32,
-                                    device=dev)
         _run(name, dev, call, q, block_idx, out, lse)
     return (out, lse) if return_lse else out
 
@@ -318,7 +326,5 @@ def copy_pages(cache: PagedKV, src, dst) -> None:
         return
     layers = cache.k.shape[0] if cache.k.ndim == 5 else 1
     _, h_kv, block, d = cache.k.shape[-4:]
-    with _lib.on_device(dev):
-        _lib.call("moba_copy_pages", *map(_lib.ptr, (cache.k, cache.v, cache.kbar, src, dst)),
-                  src.numel(), int(host), layers, pages, h_kv, block, d,
-                  _lib.DTYPE_CODE[cache.k.dtype], _lib.stream_handle(dev))
+    _lib.call_on(dev, "moba_copy_pages", *map(_lib.addr, (cache.k, cache.v, cache.kbar, src, dst)),
+                 src.numel(), host, layers, pages, h_kv, block, d, _lib.DTYPE_CODE[cache.k.dtype])

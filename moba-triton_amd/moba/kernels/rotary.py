@@ -27,17 +27,18 @@ def check_weights(q, q_weight, k_weight) -> int:
         ValueError: If a weight is not [D], or not float32 / of q's dtype, or
             the two differ in dtype.
     """
-    code = _lib.DTYPE_CODE[torch.float32]
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    for w in given:
-        if tuple(w.shape) != (q.shape[-1],):
+    found = None
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        if w.ndim != 1 or w.shape[0] != q.shape[-1]:
             raise ValueError(f"norm weight shape {tuple(w.shape)} must be ({q.shape[-1]},)")
-        if w.dtype not in (torch.float32, q.dtype):
+        if w.dtype is not torch.float32 and w.dtype is not q.dtype:
             raise ValueError(f"norm weight dtype {w.dtype} must be float32 or {q.dtype}")
-        if w.dtype != given[0].dtype:
-            raise ValueError(f"norm weight dtypes differ: {given[0].dtype}, {w.dtype}")
-        code = _lib.DTYPE_CODE[w.dtype]
-    return code
+        if found is not None and w.dtype is not found:
+            raise ValueError(f"norm weight dtypes differ: {found}, {w.dtype}")
+        found = w.dtype
+    return _lib.DTYPE_CODE[found or torch.float32]
 
 
 def check_tables(cos, sin, head_dim: int) -> int:
@@ -55,7 +56,7 @@ def check_tables(cos, sin, head_dim: int) -> int:
     if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[0] == 0:
         raise ValueError(f"cos / sin must be [positions, rotary / 2], got {tuple(cos.shape)}, "
                          f"{tuple(sin.shape)}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError(f"cos / sin must be float32, got {cos.dtype}, {sin.dtype}")
     rotary = 2 * cos.shape[1]
     if rotary % 16 or rotary > head_dim or rotary == 0:
@@ -65,48 +66,54 @@ def check_tables(cos, sin, head_dim: int) -> int:
 
 
 def _check(q, k, cos, sin, positions, q_weight, k_weight):
-    if q.ndim != 4 or k.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"shape mismatch: {tuple(q.shape)}, {tuple(k.shape)}")
-    if 0 in q.shape[2:] or 0 in k.shape[2:]:
-        raise ValueError(f"head counts and head_dim must be positive: {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}")
-    if q.dtype != k.dtype:
+    """(dtype code of the weights, rotated features)."""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[:2] != ks[:2] or qs[3] != ks[3]:
+        raise ValueError(f"shape mismatch: {tuple(qs)}, {tuple(ks)}")
+    if 0 in qs[2:] or 0 in ks[2:]:
+        raise ValueError(f"head counts and head_dim must be positive: {tuple(qs)}, {tuple(ks)}")
+    if q.dtype is not k.dtype:
         raise ValueError(f"dtype mismatch: {q.dtype}, {k.dtype}")
     if q.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"unsupported dtype {q.dtype}")
-    d = q.shape[-1]
+    d = qs[3]
     ok, reason = check_gathered_head_dim(d, q.element_size())
     if not ok:
         raise ValueError(reason)
     if d > MAX_HEAD_DIM:
         raise ValueError(f"head_dim {d} above {MAX_HEAD_DIM} is not supported")
-    check_weights(q, q_weight, k_weight)
+    code = check_weights(q, q_weight, k_weight)
     rotary = check_tables(cos, sin, d)
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if tuple(positions.shape) not in (tuple(q.shape[:2]), (q.shape[1],)):
+        if positions.shape not in (qs[:2], qs[1:2]):
             raise ValueError(f"positions shape {tuple(positions.shape)} must be "
-                             f"{tuple(q.shape[:2])} or ({q.shape[1]},)")
-    if rotary and positions is None and cos.shape[0] < q.shape[1]:
-        raise ValueError(f"cos / sin cover {cos.shape[0]} positions, the rows have {q.shape[1]}")
+                             f"{tuple(qs[:2])} or ({qs[1]},)")
+    elif rotary and cos.shape[0] < qs[1]:
+        raise ValueError(f"cos / sin cover {cos.shape[0]} positions, the rows have {qs[1]}")
+    return code, rotary
+
+
+_Strides = ctypes.c_int64 * 6
 
 
 def _shape_args(q, k, cos, code, eps, interleaved):
-    strides = (ctypes.c_int64 * 6)(*q.stride()[:3], *k.stride()[:3])
+    strides = _Strides(*q.stride()[:3], *k.stride()[:3])
     rotary, length = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
-    return [q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3], strides, rotary, length,
-            int(bool(interleaved)), float(eps), _lib.DTYPE_CODE[q.dtype], code]
+    b, s, h, d = q.shape
+    return (b, s, h, k.shape[2], d, strides, rotary, length, interleaved, eps,
+            _lib.DTYPE_CODE[q.dtype], code)
 
 
 def _forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, code):
-    dev = _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, positions)
-    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
-    if q.shape[0] * q.shape[1]:
-        with _lib.on_device(dev):
-            _lib.call("moba_norm_rotate", *map(_lib.ptr, (q, k, q_out, k_out, cos, sin, positions,
-                                                          q_weight, k_weight)),
-                      *_shape_args(q, k, cos, code, eps, interleaved), _lib.stream_handle(dev))
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    if q_out.numel():
+        a = _lib.addr
+        _lib.call_on(q.device, "moba_norm_rotate", q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
+                     k_out.data_ptr(), a(cos), a(sin), a(positions), a(q_weight), a(k_weight),
+                     *_shape_args(q, k, cos, code, eps, interleaved))
     return q_out, k_out
 
 
@@ -125,9 +132,9 @@ class NormRotateFunction(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         gq, gk = _lib.aligned_contiguous(gq), _lib.aligned_contiguous(gk)
-        dev = _lib.require_gpu(gq, gk, q, k)
+        dev = q.device
         dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
-        if not q.shape[0] * q.shape[1]:
+        if not dq.numel():
             zero = [None if w is None else torch.zeros_like(w) for w in (q_weight, k_weight)]
             return dq, dk, *zero, None, None, None, None, None, None
         dwq, dwk = (None if w is None else torch.empty(w.shape, dtype=w.dtype, device=dev)
@@ -135,11 +142,9 @@ class NormRotateFunction(torch.autograd.Function):
         size = 0 if dwq is None and dwk is None else \
             _lib.load().moba_norm_rotate_bwd_workspace_size(q.shape[-1])
         ws = torch.empty(size, device=dev, dtype=torch.uint8)
-        with _lib.on_device(dev):
-            _lib.call("moba_norm_rotate_bwd", *map(_lib.ptr, (gq, gk, q, k, dq, dk, dwq, dwk, cos,
-                                                              sin, positions, q_weight, k_weight)),
-                      *_shape_args(q, k, cos, ctx.code, ctx.eps, ctx.interleaved), _lib.ptr(ws),
-                      size, _lib.stream_handle(dev))
+        _lib.call_on(dev, "moba_norm_rotate_bwd", *map(_lib.addr, (
+            gq, gk, q, k, dq, dk, dwq, dwk, cos, sin, positions, q_weight, k_weight)),
+            *_shape_args(q, k, cos, ctx.code, ctx.eps, ctx.interleaved), ws.data_ptr(), size)
         return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 
@@ -168,15 +173,22 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
     Raises:
         ValueError: On mismatched shapes, dtypes, tables or weights.
     """
-    _check(q, k, cos, sin, positions, q_weight, k_weight)
+    code, rotary = _check(q, k, cos, sin, positions, q_weight, k_weight)
     _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, positions)
-    code = check_weights(q, q_weight, k_weight)
     q, k = _lib.aligned_rows(q), _lib.aligned_rows(k)
-    cos, sin, q_weight, k_weight = (None if t is None else _lib.aligned_contiguous(t)
-                                    for t in (cos, sin, q_weight, k_weight))
-    if positions is not None:
+    if rotary:
+        cos, sin = _lib.aligned_contiguous(cos), _lib.aligned_contiguous(sin)
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+    if positions is not None and (positions.dtype is not torch.int32 or positions.ndim != 2 or
+                                  not positions.is_contiguous()):
         positions = positions.to(torch.int32).expand(q.shape[:2]).contiguous()
-    args = (q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, code)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    args = (q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), code)
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or
+            (q_weight is not None and q_weight.requires_grad) or
+            (k_weight is not None and k_weight.requires_grad)):
         return NormRotateFunction.apply(*args)
     return _forward(*args)

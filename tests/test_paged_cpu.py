@@ -161,6 +161,7 @@ def test_library_refuses_bad_calls_on_the_host():
     assert rc(b"same number", even=2) == _lib.MOBA_ERR_INVALID
     assert rc(b"slots", take=3) == _lib.MOBA_ERR_INVALID
     assert rc(b"past blocks", take=33, slots=40) == _lib.MOBA_ERR_UNSUPPORTED
+    assert rc(b"65536 blocks", table_width=65537) == _lib.MOBA_ERR_UNSUPPORTED
     assert rc(b"null", block_table=None) == _lib.MOBA_ERR_INVALID
     assert rc(b"null", "moba_paged_attention") == _lib.MOBA_ERR_INVALID
     assert rc(b"unaligned", "moba_paged_gate", q=24, kbar=16, block_idx=16) == _lib.MOBA_ERR_INVALID
