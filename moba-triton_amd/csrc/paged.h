@@ -71,6 +71,12 @@ __device__ inline TokenAt locate(const Paged& p, int32_t tok) {
   return TokenAt{0, -1};
 }
 
+// What an address that is the same in all lanes of a wave holds, written by an
+// earlier kernel: a scalar load, which no wait for vector memory includes.
+__device__ inline int32_t uniform_load(const int32_t* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
+}
+
 // Page of block `blk` of sequence s, or -1 where the table has none.
 __device__ inline int32_t page_of(const Paged& p, int32_t s, int32_t blk) {
   if (blk >= p.width) return -1;

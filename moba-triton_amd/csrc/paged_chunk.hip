@@ -56,29 +56,51 @@ __device__ inline int32_t entry_block(const Paged& p, int32_t seq, int32_t blk) 
   return page_of(p, seq, blk) < 0 ? -1 : blk;
 }
 
+// Entries i0 + kSortThreads u of a part and kv head, kFlight of them in flight: their
+// index in the slice and their block (-1: none, or past the last of n).
+constexpr int kSortThreads = 1024;
+constexpr int kFlight = 8;
+__device__ inline void load_entries(const ChunkArgs& a, const Part& pt, int hk, int i0, int n,
+                                    int32_t (&e)[kFlight], int32_t (&blk)[kFlight]) {
+  const uint32_t group = a.h_q / a.h_kv, per = group * a.slots;
+  const int32_t* ids = a.block_idx + static_cast<int64_t>(a.t0) * a.h_q * a.slots;
+#pragma unroll
+  for (int u = 0; u < kFlight; ++u) {
+    const uint32_t i = min(i0 + kSortThreads * u, n - 1), t = i / per;
+    e[u] = ((pt.begin - a.t0 + t) * a.h_q + hk * group) * a.slots + (i - t * per);
+    blk[u] = ids[e[u]];
+  }
+#pragma unroll
+  for (int u = 0; u < kFlight; ++u) blk[u] = i0 + kSortThreads * u < n ? entry_block(a.p, pt.seq, blk[u]) : -1;
+}
+
 // counts[part, kv head, block]; dynamic LDS: width counters. grid (parts, h_kv).
-__global__ void __launch_bounds__(256) column_count_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(kSortThreads) column_count_kernel(ChunkArgs a) {
   extern __shared__ int32_t bins[];
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.n_items = 0;
   const Part pt = find_part(a.p, a.t0, a.t1, a.part, blockIdx.x);
   if (pt.seq < 0) return;
   const int hk = blockIdx.y, group = a.h_q / a.h_kv, per = group * a.slots;
-  for (int j = threadIdx.x; j < a.p.width; j += 256) bins[j] = 0;
+  for (int j = threadIdx.x; j < a.p.width; j += kSortThreads) bins[j] = 0;
   __syncthreads();
   const int n = (pt.end - pt.begin) * per;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int64_t e = (static_cast<int64_t>(pt.begin + i / per) * a.h_q + hk * group) * a.slots + i % per;
-    const int32_t blk = entry_block(a.p, pt.seq, a.block_idx[e]);
-    if (blk >= 0) atomicAdd(&bins[blk], 1);
+  for (int i0 = threadIdx.x; i0 < n; i0 += kSortThreads * kFlight) {
+    int32_t e[kFlight], blk[kFlight];
+    load_entries(a, pt, hk, i0, n, e, blk);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (blk[u] >= 0) atomicAdd(&bins[blk[u]], 1);
   }
   __syncthreads();
   int32_t* out = a.table + (static_cast<int64_t>(blockIdx.x) * a.h_kv + hk) * a.p.width;
-  for (int j = threadIdx.x; j < a.p.width; j += 256) out[j] = bins[j];
+  for (int j = threadIdx.x; j < a.p.width; j += kSortThreads) out[j] = bins[j];
 }
 
 // Per (sequence, kv head): table -> the place of every (part, block)'s first
-// entry; work items of the columns. grid (seqs, h_kv).
+// entry; work items of the columns. Dynamic LDS: width counters. grid (seqs,
+// h_kv).
 __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
+  extern __shared__ int32_t sizes[];
   __shared__ int32_t wsum[2][16];
   __shared__ int32_t base_item;
   const int32_t seq = blockIdx.x;
@@ -104,10 +126,10 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
   if (first + parts > a.parts) return;  // only where sequences claim the same tokens
   const int per = a.h_q / a.h_kv * a.slots;
   const int32_t place0 = (lo - a.t0) * a.h_q * a.slots + hk * (hi - lo) * per;
-  const int64_t row = static_cast<int64_t>(a.h_kv) * a.p.width;
+  const uint32_t row = a.h_kv * a.p.width;  // the table has at most 2^22 entries, or one part per sequence
   int32_t* table = a.table + static_cast<int64_t>(first) * row + static_cast<int64_t>(hk) * a.p.width;
   const int32_t blocks = min(a.p.width, (r.len + a.p.block - 1) / a.p.block);
-  // Two rounds over the columns: the number of items, then the lists.
+  // The columns' entries into LDS, and the number of items; then the lists.
   int32_t items = 0;
   for (int round = 0; round < 2; ++round) {
     int32_t carry_e = 0, carry_i = 0;
@@ -115,7 +137,19 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
       const int32_t b = b0 + threadIdx.x;
       int32_t n = 0;
       if (b < blocks) {
-        for (int32_t q = 0; q < parts; ++q) n += table[q * row + b];
+        if (round == 0) {
+          const int32_t* p = table + b;
+          for (int32_t q0 = 0; q0 < parts; q0 += 8) {
+            int32_t x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = p[static_cast<int64_t>(min(q0 + u, parts - 1)) * row];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n += q0 + u < parts ? x[u] : 0;
+          }
+          sizes[b] = n;
+        } else {
+          n = sizes[b];
+        }
       }
       const int32_t k = (n + kItem - 1) / kItem;
       int32_t ie = n, ii = k;
@@ -127,24 +161,30 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
       if (lane == 63) { wsum[0][wave] = ie; wsum[1][wave] = ii; }
       __syncthreads();
       int32_t te = 0, ti = 0;
-#pragma unroll
       for (int w = 0; w < 16; ++w) {
         if (w < wave) { ie += wsum[0][w]; ii += wsum[1][w]; }
         te += wsum[0][w];
         ti += wsum[1][w];
       }
       __syncthreads();
-      if (round == 1 && b < blocks) {
+      if (round == 1 && b < blocks && n) {
         int32_t at = place0 + carry_e + ie - n;
-        const int32_t start = at;
-        for (int32_t q = 0; q < parts; ++q) {
-          const int32_t c = table[q * row + b];
-          table[q * row + b] = at;
-          at += c;
-        }
         const int32_t i0 = base_item + carry_i + ii - k;
         for (int32_t i = 0; i < k && i0 + i < a.max_items; ++i)
-          a.items[i0 + i] = make_int4(seq * a.h_kv + hk, b, start + i * kItem, min(kItem, n - i * kItem));
+          a.items[i0 + i] = make_int4(seq * a.h_kv + hk, b, at + i * kItem, min(kItem, n - i * kItem));
+        int32_t* p = table + b;
+        for (int32_t q0 = 0; q0 < parts; q0 += 8) {
+          int32_t x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[u] = p[static_cast<int64_t>(min(q0 + u, parts - 1)) * row];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            if (q0 + u < parts) {
+              p[static_cast<int64_t>(q0 + u) * row] = at;
+              at += x[u];
+            }
+          }
+        }
       }
       carry_e += te;
       carry_i += ti;
@@ -159,23 +199,25 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
 
 // Entries to their places; those that attend to nothing leave (m, l) = (-inf,
 // 0). Dynamic LDS: width cursors. grid (parts, h_kv).
-__global__ void __launch_bounds__(256) column_place_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(kSortThreads) column_place_kernel(ChunkArgs a) {
   extern __shared__ int32_t cursor[];
   const Part pt = find_part(a.p, a.t0, a.t1, a.part, blockIdx.x);
   if (pt.seq < 0) return;
   const int hk = blockIdx.y, group = a.h_q / a.h_kv, per = group * a.slots;
   const int32_t* row = a.table + (static_cast<int64_t>(blockIdx.x) * a.h_kv + hk) * a.p.width;
-  for (int j = threadIdx.x; j < a.p.width; j += 256) cursor[j] = row[j];
+  for (int j = threadIdx.x; j < a.p.width; j += kSortThreads) cursor[j] = row[j];
   __syncthreads();
   const int n = (pt.end - pt.begin) * per;
-  const int64_t e0 = static_cast<int64_t>(a.t0) * a.h_q * a.slots;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int64_t e = (static_cast<int64_t>(pt.begin + i / per) * a.h_q + hk * group) * a.slots + i % per;
-    const int32_t blk = entry_block(a.p, pt.seq, a.block_idx[e]);
-    if (blk >= 0)
-      a.entries[atomicAdd(&cursor[blk], 1)] = static_cast<int32_t>(e - e0);
-    else
-      *reinterpret_cast<float2*>(a.part_ml + 2 * (e - e0)) = make_float2(-INFINITY, 0.f);
+  for (int i0 = threadIdx.x; i0 < n; i0 += kSortThreads * kFlight) {
+    int32_t e[kFlight], blk[kFlight];
+    load_entries(a, pt, hk, i0, n, e, blk);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      if (blk[u] >= 0)
+        a.entries[atomicAdd(&cursor[blk[u]], 1)] = e[u];
+      else if (i0 + kSortThreads * u < n)
+        *reinterpret_cast<float2*>(a.part_ml + 2 * static_cast<int64_t>(e[u])) = make_float2(-INFINITY, 0.f);
+    }
   }
 }
 
@@ -209,6 +251,29 @@ __device__ inline void load_to_lds(const void* src, void* dst) {
       (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
+// Waits until at most N of the wave's vector memory operations are under way
+// (they end in order). Loads to LDS count as such: a barrier alone does not
+// wait for them.
+template <int N>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// A barrier that waits for no vector memory (__syncthreads waits for every
+// load to LDS under way): each wave waits for its own before.
+__device__ inline void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// 4 bytes each: lane i's to `dst` + 4 i.
+__device__ inline void load_word_to_lds(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(
+      reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
+      (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+
 // KT tiles of 32 keys cover the block. A wave holds 32 entries, one per lane
 // pair (lane, lane ^ 32):
 //   S^T[key][entry] = K . Q^T,   O^T[feature][entry] = V^T . P^T
@@ -227,65 +292,137 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   constexpr int DT = D / 32;
   __shared__ __attribute__((aligned(16))) uint16_t Ks[KEYS * D];
   __shared__ __attribute__((aligned(16))) uint16_t Vs[KEYS * D];
+  __shared__ int32_t s_ent[2][4][64];
+  __shared__ int s_bad;  // the values hold infinities or NaN
+  constexpr int LOADS = KEYS * RQ / 256;  // per thread, for the keys or the values
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = lane >> 5, col = lane & 31;
   const int n_items = min(*a.n_items, a.max_items);
   const uint16_t* Q = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(a.t0) * a.h_q * D;
-  for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-    const int4 it = a.items[item];
-    const int32_t seq = it.x / a.h_kv;
-    const int hk = it.x - seq * a.h_kv;
-    const NewTokens nt = new_tokens(a.p, seq);
-    const int64_t key0 = static_cast<int64_t>(it.y) * a.p.block;
-    const int key_lim = static_cast<int>(min(static_cast<int64_t>(a.p.block), nt.len - key0));
-    const int32_t page = max(page_of(a.p, seq, it.y), 0);
+
+  // A work item: where its block lies, and this lane's entry. What all lanes
+  // share comes by scalar loads.
+  struct Item {
+    const uint16_t *k, *v;
+    int count;     // entries
+    int key_lim;   // keys up to the sequence's end
+    int32_t pos0;  // position of the slice's first token (as if of this sequence), from the block's first key
+    bool masked;   // some new token does not see all KEYS keys
+    const int32_t* entries;
+  };
+  auto describe = [&](int item) {
+    const int32_t* it = reinterpret_cast<const int32_t*>(a.items + item);
+    const int32_t x = uniform_load(it), blk = uniform_load(it + 1), place = uniform_load(it + 2);
+    const int32_t seq = x / a.h_kv;
+    const int hk = x - seq * a.h_kv;
+    const int32_t first = a.p.cu ? uniform_load(a.p.cu + seq) : seq * a.p.even;
+    const int32_t end = a.p.cu ? uniform_load(a.p.cu + seq + 1) : first + a.p.even;
+    const int32_t len = uniform_load(a.p.seq_lens + seq);
+    int32_t page = uniform_load(a.p.table + static_cast<int64_t>(seq) * a.p.width + blk);
+    page = page >= 0 && page < a.p.pages ? page : 0;
     const int64_t base = (static_cast<int64_t>(page) * a.h_kv + hk) * a.p.block * D;
-    const uint16_t* kg = static_cast<const uint16_t*>(a.k) + base;
-    const uint16_t* vg = static_cast<const uint16_t*>(a.v) + base;
-    // Rows past the sequence's end read its last one; their weights are 0.
-#pragma unroll
-    for (int u = 0; u < KEYS * RQ / 256; ++u) {
-      const int i = u * 256 + tid, row = i / RQ, piece = i % RQ;
-      load_to_lds(kg + min(row, key_lim - 1) * D + 8 * (piece ^ swizzle_k<D>(row)),
-                  &Ks[(u * 256 + wave * 64) * 8]);
-    }
-#pragma unroll
-    for (int u = 0; u < KEYS * RQ / 256; ++u) {
-      const int i = u * 256 + tid, row = i / RQ, piece = i % RQ;
-      load_to_lds(vg + min(row, key_lim - 1) * D + 8 * (piece ^ swizzle_v<D>(row)),
-                  &Vs[(u * 256 + wave * 64) * 8]);
-    }
+    const int32_t key0 = blk * a.p.block;  // below len
+    Item d;
+    d.k = static_cast<const uint16_t*>(a.k) + base;
+    d.v = static_cast<const uint16_t*>(a.v) + base;
+    d.count = uniform_load(it + 3);
+    d.key_lim = min(a.p.block, len - key0);
+    d.pos0 = len - end + a.t0 - key0;
+    d.masked = d.key_lim < KEYS || d.pos0 + max(first - a.t0, 0) < KEYS - 1;
+    d.entries = a.entries + place;
+    return d;
+  };
+  // Lanes' entries (the first one where a lane has none) of every other item.
+  // By way of LDS: the compiler would wait for the values under way as well
+  // when it copies a register that a load fills.
+  auto load_entries = [&](const Item& d, int odd) {
     const int mine = wave * 32 + col;
-    const bool live = mine < it.w;
-    const int32_t ent = a.entries[it.z + (live ? mine : 0)];
-    const int32_t qrow = ent / a.slots;
-    V8 bq[D / 16];
+    load_word_to_lds(d.entries + (mine < d.count ? mine : 0), &s_ent[odd][wave][0]);
+  };
+  // Rows past the sequence's end hold anything, their weights are 0. Rows past
+  // the page (blocks that are no multiple of 32) read its last one.
+  constexpr int ROWS = 256 / RQ;  // rows per load; the swizzles repeat every 16
+  const uint32_t row0 = tid / RQ, piece = tid % RQ;
+  const uint32_t last = a.p.block - 1;
+  auto load_rows = [&](const uint16_t* src, uint16_t* dst, uint32_t swizzled) {
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k)
-      bq[k] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
-                                         Q + static_cast<int64_t>(qrow) * D + 16 * k + 8 * h));
-    const int32_t pos = nt.len - nt.n + (a.t0 + qrow / a.h_q - nt.first);
-    const int64_t row_lim = pos - key0;
-    const int lim = live ? static_cast<int>(min(static_cast<int64_t>(key_lim - 1), row_lim)) : -1;
-    // Loads to LDS count as vector memory: a barrier alone does not wait for them.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (wave * 32 < it.w) {
-      floatx16_t s[KT];
+    for (int u = 0; u < LOADS; ++u) {
+      uint32_t row = u * ROWS + row0;
+      if ((u + 1) * ROWS > 32 * (KT - 1)) row = min(row, last);
+      load_to_lds(src + (row * D + swizzled), dst + (u * 256 + wave * 64) * 8);
+    }
+  };
+  auto load_keys = [&](const Item& d) { load_rows(d.k, Ks, 8 * (piece ^ swizzle_k<D>(row0))); };
+  auto load_values = [&](const Item& d) { load_rows(d.v, Vs, 8 * (piece ^ swizzle_v<D>(row0))); };
+  V8 bq[D / 16];
+  auto load_query = [&](int32_t ent) {
+    const uint16_t* q = Q + static_cast<int64_t>(ent / a.slots) * D + 8 * h;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) bq[k] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(q + 16 * k));
+  };
+
+  // LDS addresses: of the keys' operands by K-step (tiles 32 rows apart), of
+  // the values' by feature tile (steps of 16 keys apart; the swizzle of a row
+  // depends on its place among 16).
+  const uint16_t* ka[D / 16];
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) ka[k] = &Ks[col * D + 8 * ((2 * k + h) ^ swizzle_k<D>(col))];
+  const uint16_t *va0[DT], *va1[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int key = 4 * h + ((lane & 15) >> 2);
+    const int piece = dt * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    va0[dt] = &Vs[key * D + 8 * (piece ^ swizzle_v<D>(key)) + 4 * (lane & 1)];
+    va1[dt] = &Vs[(key + 8) * D + 8 * (piece ^ swizzle_v<D>(key + 8)) + 4 * (lane & 1)];
+  }
+
+  // One item ahead: its queries and keys are on their way from when this
+  // item's first product is done, its values from when the second is. The
+  // entries of the one after it are asked for before those, so that the waits
+  // below, which count, include them.
+  int item = blockIdx.x;
+  if (item >= n_items) return;
+  const int stride = static_cast<int>(gridDim.x);
+  Item d = describe(item), next = describe(min(item + stride, n_items - 1));
+  load_entries(d, 0);
+  load_entries(next, 1);
+  wait_loads<0>();
+  load_query(s_ent[0][wave][lane]);
+  load_keys(d);
+  load_values(d);
+  for (int odd = 0;; odd ^= 1) {
+    const bool more = item + stride < n_items;
+    const bool work = wave * 32 < d.count;
+    const bool live = wave * 32 + col < d.count;
+    const int32_t ent = s_ent[odd][wave][lane];
+    const int lim = live ? min(d.key_lim - 1, d.pos0 + ent / a.slots / a.h_q) : -1;  // last key seen
+    wait_loads<LOADS>();  // all but the values
+    meet();
+    if (tid == 0) s_bad = 0;
+    floatx16_t s[KT];
+    if (work) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) s[kt] = floatx16_t{};
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const int row = kt * 32 + col;
-          const V8 ka = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
-                                                   &Ks[row * D + 8 * ((2 * k + h) ^ swizzle_k<D>(row))]));
-          s[kt] = M::mma(ka, bq[k], s[kt]);
-        }
+        for (int kt = 0; kt < KT; ++kt)
+          s[kt] = M::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(ka[k] + kt * 32 * D)), bq[k], s[kt]);
+    }
+    meet();  // every wave is done with the keys
+    Item after = next;
+    if (more) {
+      after = describe(min(item + 2 * stride, n_items - 1));
+      const int32_t next_ent = s_ent[odd ^ 1][wave][lane];
+      load_entries(after, odd);
+      load_query(next_ent);
+      load_keys(next);
+    }
+    const bool whole = __all(!live || lim == KEYS - 1);
+    float m = -INFINITY, l = 0.f;
+    V8 bp[KEYS / 16];
+    if (work) {
       // s[kt][v] is key 32 kt + 8 (v / 4) + 4 h + v % 4.
-      const bool whole = __all(!live || lim == KEYS - 1);
-      float m = -INFINITY, l = 0.f;
       if (!whole) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -310,20 +447,47 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
           l += p;
         }
       l += __shfl_xor(l, 32);
-      V8 bp[KEYS / 16];
 #pragma unroll
       for (int j = 0; j < KEYS / 16; ++j)
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           bp[j][u] = static_cast<typename M::scalar>(s[j >> 1][8 * (j & 1) + u]);
+    }
+    if (more)
+      wait_loads<LOADS>();  // all but the next keys
+    else
+      wait_loads<0>();
+    meet();
+    // A weight of 0 times an infinite or NaN value is NaN, but a value that a
+    // query does not see must not reach it. Where the block has hidden keys,
+    // such values are taken out, and put back after the product for the
+    // queries that see them.
+    bool bad = false;
+    if (d.masked) {
+      u32x4 x[LOADS];
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) x[u] = *reinterpret_cast<const u32x4*>(&Vs[(u * 256 + tid) * 8]);
+      uint32_t found = 0;
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          found |= (x[u][w] & M::kInf) == M::kInf ? 1u : 0u;
+          found |= ((x[u][w] >> 16) & M::kInf) == M::kInf ? 1u : 0u;
+        }
+      if (found) s_bad = 1;
+      meet();
+      bad = s_bad != 0;
+      if (bad) {
+        for (int i = tid * 8; i < KEYS * D; i += 256 * 8)
+          for (int e = 0; e < 8; ++e)
+            if ((Vs[i + e] & M::kInf) == M::kInf) Vs[i + e] = 0;
+        meet();
+      }
+    }
+    if (work) {
       // Value operand of features 32 dt + [0, 32) and keys 16 j + [0, 16).
-      auto values = [&](int j, int dt) {
-        const int key = 16 * j + 4 * h + ((lane & 15) >> 2);
-        const int piece = dt * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        const uint16_t* p0 = &Vs[key * D + 8 * (piece ^ swizzle_v<D>(key)) + 4 * (lane & 1)];
-        const uint16_t* p1 = &Vs[(key + 8) * D + 8 * (piece ^ swizzle_v<D>(key + 8)) + 4 * (lane & 1)];
-        return transposed<V8>(p0, p1);
-      };
+      auto values = [&](int j, int dt) { return transposed<V8>(va0[dt] + j * 16 * D, va1[dt] + j * 16 * D); };
       floatx16_t o[DT];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] = floatx16_t{};
@@ -331,47 +495,22 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
       for (int j = 0; j < KEYS / 16; ++j)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = M::mma(values(j, dt), bp[j], o[dt]);
-      if (!whole) {
-        // A weight of 0 times an infinite or NaN value is NaN, but a value
-        // that a query does not see must not reach it. Where any result is
-        // not finite: the product again without such values, and who sees
-        // which of them by two more products of zeros and ones.
-        float bad = 0.f;
+      if (bad) {
+        // What the queries see of the values that were taken out.
+        for (int key = 0; key < d.key_lim; ++key) {
+          const uint16_t* row = d.v + key * D + 4 * h;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) bad = fmaf(o[dt][v], 0.f, bad);
-        if (__any(bad != 0.f)) {
-          using S = typename M::scalar;
-          for (int dt = 0; dt < DT; ++dt) {
-            floatx16_t fin = floatx16_t{}, up = floatx16_t{}, down = floatx16_t{};
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const u32x2 x = *reinterpret_cast<const u32x2*>(row + dt * 32 + 8 * q4);
 #pragma unroll
-            for (int j = 0; j < KEYS / 16; ++j) {
-              const V8 va = values(j, dt);
-              V8 f, pu, nu, see;
-#pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                const uint32_t bits = __builtin_bit_cast(uint16_t, va[u]);
-                const bool inf = (bits & 0x7fffu) == M::kInf, nan = (bits & 0x7fffu) > M::kInf;
-                f[u] = inf || nan ? static_cast<S>(0.f) : va[u];
-                pu[u] = static_cast<S>(nan || (inf && !(bits & 0x8000u)) ? 1.f : 0.f);
-                nu[u] = static_cast<S>(nan || (inf && (bits & 0x8000u)) ? 1.f : 0.f);
-                const int key = 16 * j + 8 * (u >> 2) + 4 * h + (u & 3);
-                see[u] = static_cast<S>(key <= lim ? 1.f : 0.f);
+              for (int w = 0; w < 4; ++w) {
+                const uint16_t bits = static_cast<uint16_t>(x[w >> 1] >> (16 * (w & 1)));
+                if ((bits & M::kInf) == M::kInf && key <= lim)
+                  o[dt][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
               }
-              fin = M::mma(f, bp[j], fin);
-              up = M::mma(pu, see, up);
-              down = M::mma(nu, see, down);
             }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const float x = up[v] > 0.f ? INFINITY : 0.f, y = down[v] > 0.f ? INFINITY : 0.f;
-              fin[v] += x - y;
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-              if (d == dt) o[d] = fin;
-          }
         }
       }
       if (live) {
@@ -389,7 +528,12 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
           }
       }
     }
-    __syncthreads();  // every wave is done with the staged rows
+    meet();  // every wave is done with the values
+    if (!more) break;
+    load_values(next);
+    d = next;
+    next = after;
+    item += stride;
   }
 }
 
@@ -404,27 +548,50 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
     const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * a.h_q + hd) * a.slots;
     const float* ml = a.part_ml + 2 * e0;
     const u32x4* acc = static_cast<const u32x4*>(a.part_acc) + e0 * LPR + c;
-    float top = -INFINITY;
-    for (int j = 0; j < a.slots; ++j) top = fmaxf(top, ml[2 * j]);
-    const float z = top > -INFINITY ? top : 0.f;
-    float total = 0.f, o[8];
+    // Eight slots in flight. Those that were not written (m = -inf) hold
+    // anything: they count as zeros.
+    float top = -INFINITY, total = 0.f, o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    for (int j = 0; j < a.slots; ++j) {
-      const float m = ml[2 * j];
-      if (m == -INFINITY) continue;  // nothing was written there
-      const float w = __builtin_amdgcn_exp2f(m - z);
-      total = fmaf(ml[2 * j + 1], w, total);
-      const u32x4 raw = acc[j * LPR];
-      const T* x = reinterpret_cast<const T*>(&raw);
+    for (int j0 = 0; j0 < a.slots; j0 += 8) {
+      float2 x[8];
+      u32x4 raw[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = fmaf(Elem<T>::load(x, e), w, o[e]);
+      for (int u = 0; u < 8; ++u) {
+        const int j = min(j0 + u, a.slots - 1);
+        x[u] = *reinterpret_cast<const float2*>(ml + 2 * j);
+        raw[u] = acc[j * LPR];
+      }
+      float m = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (j0 + u >= a.slots) x[u].x = -INFINITY;
+        m = fmaxf(m, x[u].x);
+      }
+      const float z = m > -INFINITY ? m : 0.f;
+      const float old = __builtin_amdgcn_exp2f(top - z);
+      total *= old;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= old;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const bool in = x[u].x != -INFINITY;
+        const float w = __builtin_amdgcn_exp2f(x[u].x - z);
+        total = fmaf(in ? x[u].y : 0.f, w, total);
+        const u32x4 r = in ? raw[u] : u32x4{0, 0, 0, 0};
+        const T* v = reinterpret_cast<const T*>(&r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(Elem<T>::load(v, e), w, o[e]);
+      }
+      top = m;
     }
     const int64_t row = static_cast<int64_t>(tok) * a.h_q + hd;
     T* out = static_cast<T*>(a.out) + row * D + 8 * c;
+    T y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      Elem<T>::store(out, e, total > 0.f ? o[e] / total : (total == 0.f ? 0.f : o[e] + total));
+      Elem<T>::store(y, e, total > 0.f ? o[e] / total : (total == 0.f ? 0.f : o[e] + total));
+    *reinterpret_cast<u32x4*>(out) = __builtin_bit_cast(u32x4, y);
     if (a.lse && c == 0)
       a.lse[hd * static_cast<int64_t>(a.p.tokens) + tok] =
           total > 0.f ? top + log2f(total) : (total == 0.f ? -INFINITY : total);
@@ -437,7 +604,7 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 bool chunk_takes(const moba_paged& c) {
   return c.dtype != MOBA_FP32 && (c.head_dim == 64 || c.head_dim == 128) && c.block_size <= 128 &&
-         c.table_width <= 16384 && c.h_kv <= 65535 && c.tokens >= 4 * c.seqs;
+         c.table_width <= 15360 && c.h_kv <= 65535 && c.tokens >= 4 * c.seqs;
 }
 
 ChunkPlan chunk_plan(const moba_paged& c) {
@@ -446,8 +613,9 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   // Partial rows of at most 2^29 bytes at a time.
   pl.slice = (int64_t(1) << 29) / (per_token * c.head_dim * 2);
   pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
-  // Parts of 64 tokens, more where the count table would pass 2^22 entries.
-  pl.part = 64;
+  // Parts of 256 tokens (64: the scan over 32 parts of 2048 tokens took 22 us,
+  // over 8 parts 9), more where the count table would pass 2^22 entries.
+  pl.part = 256;
   const int64_t row = c.h_kv * c.table_width;
   while (pl.part < pl.slice && (pl.slice / pl.part + c.seqs) * row > (int64_t(1) << 22)) pl.part *= 2;
   pl.parts = cdiv(pl.slice, pl.part) + c.seqs;
@@ -494,10 +662,10 @@ int chunk_attend(const moba_paged& c, const Paged& p, void* workspace, hipStream
   for (int64_t t0 = 0; t0 < c.tokens; t0 += pl.slice) {
     a.t0 = static_cast<int32_t>(t0);
     a.t1 = static_cast<int32_t>(c.tokens - t0 < pl.slice ? c.tokens : t0 + pl.slice);
-    hipLaunchKernelGGL(column_count_kernel, parts, dim3(256), lds, s, a);
+    hipLaunchKernelGGL(column_count_kernel, parts, dim3(kSortThreads), lds, s, a);
     hipLaunchKernelGGL(column_scan_kernel, dim3(static_cast<unsigned>(c.seqs), static_cast<unsigned>(c.h_kv)),
-                       dim3(1024), 0, s, a);
-    hipLaunchKernelGGL(column_place_kernel, parts, dim3(256), lds, s, a);
+                       dim3(1024), lds, s, a);
+    hipLaunchKernelGGL(column_place_kernel, parts, dim3(kSortThreads), lds, s, a);
     int st = check_launch("moba_paged_attend (columns)");
     if (st) return st;
     auto attend = [&](auto t, auto dim, auto kt) {

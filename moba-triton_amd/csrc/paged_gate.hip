@@ -112,30 +112,38 @@ __global__ void __launch_bounds__(256) select_kernel(GateArgs a) {
 // ---------------------------------------------------------------------------
 // Many queries, 16-bit types. A wave holds 32 queries (tokens by the query
 // heads of one kv head), two lanes each; the representatives pass through LDS
-// 64 at a time, and a 32x32x16 MFMA chain leaves each lane 16 approximate
-// scores of its query. |approximate - exact| <= E: the products are exact in
-// float32, D additions round by at most a unit of the last place each
-// (truncation included) of sums of at most |q| |kbar|; and what the unit may
-// flush below the normal range.
+// 64 at a time, and two 32x32x16 MFMA chains leave each lane 2 x 16
+// approximate scores of its query. |approximate - exact| <= E: the products
+// are exact in float32, D additions round by at most a unit of the last place
+// each (truncation included) of sums of at most |q| |kbar|. (The unit keeps
+// subnormal inputs of both types, as it does subnormal float32 results: 16
+// products of 2^-24 and 1 in fp16, of 2^-130 and 2^10 in bf16, of 2^-100 and
+// 2^-40, come out exact.)
 //
-// Each lane keeps the best M of its blocks by (largest key the score can
-// have, id), a key being the score rounded to the type. An entry whose
-// smallest key is the same is certain, the others are marked. At the end a
-// lane forms the exact scores of its marked entries, as far down as `take`
-// certain ones do not stand above them, and the two lists are ranked. What
-// left a list has no larger key than its last entry had, so the result stands
-// where the last chosen entry ranks no lower than both lists' last; the other
-// queries (constructed ties, infinities, NaN) score every block exactly.
+// Two passes over the blocks. The first keeps the largest of each lane's 16
+// scores per tile, the best K of those: the take-th of both lanes' lists is a
+// score that `take` blocks reach, so whatever cannot round to its key is out.
+// The second writes the scores that can to a small buffer per lane (a few per
+// query; one pass that keeps sorted lists as it goes spends 168 us on the
+// lists where this spends 50, below). A full buffer goes into the lane's list
+// of the best M by (largest key the score can have, id), a key being the
+// score rounded to the type, and the list's last entry then bounds what comes.
 //
-// Bound by the list work: [2048 tokens, 32/8 heads of 128, 1008 blocks] is 17
-// GFLOP of products, tens of instructions per kept score.
+// An entry whose smallest key is its largest is certain, the others are
+// marked. At the end a lane forms the exact scores of its marked entries, as
+// far down as `take` certain ones do not stand above them, and the two lists
+// are ranked. What left a list has no larger key than its last entry had, so
+// the result stands where the last chosen entry ranks no lower than both
+// lists' last; the other queries (constructed ties, infinities, NaN) score
+// every block exactly.
 constexpr int kNormParts = 16;
 
 template <typename T> struct GateUnit;
 template <> struct GateUnit<bf16_t> {
   typedef bf16x8_t vec;
-  static constexpr float kFlush = 1.2e-38f;  // inputs below it may count as 0
   static constexpr float kLowest = -3.3961514e38f;  // rounds to -inf, as all below it
+  static constexpr float kUnit = 0.008f;            // above the largest relative unit, 2^-7
+  static constexpr float kSmall = 1e-37f;           // above the smallest absolute one
   __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -148,8 +156,9 @@ template <> struct GateUnit<bf16_t> {
 };
 template <> struct GateUnit<f16_t> {
   typedef f16x8_t vec;
-  static constexpr float kFlush = 6.2e-5f;
   static constexpr float kLowest = -65520.f;
+  static constexpr float kUnit = 0.001f;
+  static constexpr float kSmall = 1e-7f;
   __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -220,25 +229,33 @@ __device__ inline uint32_t exact_key(const T* q, const T* kb) {
   return score_key<Rank<T>>(Elem<T>::round(static_cast<float>(t)));
 }
 
-// A query's blocks all scored exactly, by one wave.
+// A query's blocks all scored exactly, by one wave. Arguments by value: a
+// reference would put the caller's copy into scratch memory.
 template <typename T, int D, int TM>
-__device__ __attribute__((noinline)) void exact_query(const GateArgs& a, int32_t seq, int32_t own, int hk,
-                                                      const T* q, int32_t* out) {
+__device__ __attribute__((noinline)) void exact_query(const int32_t* pages, int32_t n_pages, int32_t past,
+                                                      const T* kbar, int64_t page_stride, const T* q,
+                                                      int take, int32_t own, int slots, int32_t* out) {
   WaveBest<Rank<T>, TM> list;
   list.clear();
-  const int32_t past = min(own, a.p.width);
   for (int32_t j = threadIdx.x & 63; j < past; j += 64) {
-    const int32_t page = page_of(a.p, seq, j);
-    if (page >= 0)
-      list.add(list.word(
-          exact_key<T, D>(q, static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D), j));
+    const int32_t page = pages[j];
+    if (page >= 0 && page < n_pages) list.add(list.word(exact_key<T, D>(q, kbar + page * page_stride), j));
   }
   list.meet();
-  list.emit(a.take, own_entry(a.p, a.current, seq, own), a.slots, out);
+  list.emit(take, own, slots, out);
 }
 
-template <typename T, int D, int M, int TM>
-__global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
+// What a wave's lanes wrote to LDS, visible to its other lanes.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+constexpr int kBuffer = 24;  // entries per lane
+
+template <typename T, int D, int M, int K>
+__global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
   using U = GateUnit<T>;
   using V8 = typename U::vec;
   constexpr int RQ = D / 8;     // 16-byte pieces per row
@@ -247,6 +264,9 @@ __global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t rows[2][ROWS * D];
   __shared__ int32_t s_page[2][ROWS];
   __shared__ uint64_t s_valid[4];
+  constexpr int kHeld = M > kBuffer ? M : kBuffer;
+  __shared__ float s_score[4][kHeld][64];
+  __shared__ uint16_t s_id[4][kHeld][64];
   const Part pt = find_part(a.p, 0, a.p.tokens, a.tile_tokens, blockIdx.x);
   if (pt.seq < 0) return;
   const NewTokens nt = new_tokens(a.p, pt.seq);
@@ -284,8 +304,7 @@ __global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
     kn = u2f(best) * 1.0001f;
   }
   // Widened by the rounding of a -+ E itself, with |a| * 2.4e-7 below.
-  const float E = (qn * kn * (D * 0x1p-23f) + U::kFlush * sqrtf(static_cast<float>(D)) * (qn + kn) +
-                   (D + 1) * 1.2e-38f) * 1.001f;
+  const float E = (qn * kn * (D * 0x1p-23f) + (D + 1) * 1.2e-38f) * 1.001f;
   const bool bounded = qn * kn < 3e38f && E < 3e38f;  // false for infinities and NaN
 
   // Pages of stage st, by wave 0: to LDS, with a bit for each that is one.
@@ -314,82 +333,165 @@ __global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
   uint32_t key[M];
 #pragma unroll
   for (int i = 0; i < M; ++i) key[i] = 0;
-  float floor_value = U::kLowest;  // scores that round to at most this cannot enter the list
-  if (stages > 0) {
+  float tops[K];  // pass 0: the best tile maxima, best first
+#pragma unroll
+  for (int i = 0; i < K; ++i) tops[i] = -INFINITY;
+  float floor_value = U::kLowest;  // pass 1: scores that round to at most this are out
+  int held = 0;                    // entries in the lane's buffer
+  float* score = &s_score[wave][0][lane];  // entry i at [64 i]
+  uint16_t* id = &s_id[wave][0][lane];
+  // The buffer into the list.
+  auto fold = [&]() {
+    for (int i = 0; __any(i < held); ++i) {
+      const float x = score[64 * i];
+      const uint32_t top = U::bits(fmaf(fabsf(x), 2.4e-7f, x) + E);
+      const uint32_t low = U::bits(fmaf(-fabsf(x), 2.4e-7f, x) - E);
+      uint32_t e = ordered(top) | (0x7fffu - id[64 * i]) << 1 | (top != low ? 1u : 0u);
+      e = i < held ? e : 0u;
+#pragma unroll
+      for (int p = M - 1; p > 0; --p) key[p] = med3(key[p - 1], key[p], e);
+      key[0] = max(key[0], e);
+    }
+    held = 0;
+    if (key[M - 1]) floor_value = fmaxf(floor_value, U::value(unordered(key[M - 1])));
+  };
+  for (int pass = 0; pass < 2 && stages > 0; ++pass) {
+    __syncthreads();  // the previous pass is done with the stages
     if (wave == 0) {
       put_pages(0, page_at(0));
       if (stages > 1) put_pages(1, page_at(1));
     }
     __syncthreads();
     stage(0);
-  }
-  for (int st = 0; st < stages; ++st) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int32_t ahead = -1;
-    if (wave == 0 && st + 2 < stages) ahead = page_at(st + 2);
-    if (st + 1 < stages) stage(st + 1);
-    if (busy) {
-      const uint64_t valid = s_valid[st & 3];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int32_t j0 = st * ROWS + half * 32;
-        if (j0 >= horizon) break;
-        floatx16_t s = floatx16_t{};
-        const int row = half * 32 + (lane & 31);
-        const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
+    for (int st = 0; st < stages; ++st) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      int32_t ahead = -1;
+      if (wave == 0 && st + 2 < stages) ahead = page_at(st + 2);
+      if (st + 1 < stages) stage(st + 1);
+      if (busy) {
+        const uint64_t valid = s_valid[st & 3];
+        floatx16_t s[2] = {floatx16_t{}, floatx16_t{}};
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          s = U::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
-                                                &rows[st & 1][row * D + 8 * ((2 * k + h) ^ swz)])),
-                     bq[k], s);
-        const uint32_t ok = static_cast<uint32_t>(valid >> (32 * half));
-        if (j0 + 32 > sure || ok != 0xffffffffu) {  // some blocks are not for every query
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int o = 8 * (v >> 2) + 4 * h + (v & 3);
-            if (j0 + o >= past || !((ok >> o) & 1u)) s[v] = -INFINITY;
+          for (int half = 0; half < 2; ++half) {
+            const int row = half * 32 + (lane & 31);
+            const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
+            s[half] = U::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
+                                                        &rows[st & 1][row * D + 8 * ((2 * k + h) ^ swz)])),
+                             bq[k], s[half]);
+          }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int32_t j0 = st * ROWS + half * 32;
+          if (j0 >= horizon) continue;
+          const uint32_t ok = static_cast<uint32_t>(valid >> (32 * half));
+          if (j0 + 32 > sure || ok != 0xffffffffu) {  // some blocks are not for every query
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int o = 8 * (v >> 2) + 4 * h + (v & 3);
+              if (j0 + o >= past || !((ok >> o) & 1u)) s[half][v] = -INFINITY;
+            }
+          }
+          float most = s[half][0];
+#pragma unroll
+          for (int v = 1; v < 16; ++v) most = fmaxf(most, s[half][v]);
+          if (pass == 0) {
+#pragma unroll
+            for (int i = K - 1; i > 0; --i) tops[i] = __builtin_amdgcn_fmed3f(tops[i - 1], tops[i], most);
+            tops[0] = fmaxf(tops[0], most);
+          } else if (__any(fmaf(fabsf(most), 2.4e-7f, most) + E > floor_value)) {
+            if (__any(held > kBuffer - 16)) fold();
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const float x = s[half][v];
+              if (fmaf(fabsf(x), 2.4e-7f, x) + E > floor_value) {
+                score[64 * held] = x;
+                id[64 * held] = static_cast<uint16_t>(j0 + 8 * (v >> 2) + 4 * h + (v & 3));
+                ++held;
+              }
+            }
           }
         }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float x = s[v];
-          const float hi = fmaf(fabsf(x), 2.4e-7f, x) + E;
-          if (hi > floor_value) {
-            const uint32_t top = U::bits(hi);
-            const uint32_t low = U::bits(fmaf(-fabsf(x), 2.4e-7f, x) - E);
-            const uint32_t j = static_cast<uint32_t>(j0 + 8 * (v >> 2) + 4 * h + (v & 3));
-            const uint32_t e = ordered(top) | (0x7fffu - j) << 1 | (top != low ? 1u : 0u);
-#pragma unroll
-            for (int i = M - 1; i > 0; --i) key[i] = med3(key[i - 1], key[i], e);
-            key[0] = max(key[0], e);
-          }
-        }
-        floor_value = key[M - 1] ? U::value(unordered(key[M - 1])) : U::kLowest;
       }
+      if (wave == 0 && st + 2 < stages) put_pages(st + 2, ahead);
     }
-    if (wave == 0 && st + 2 < stages) put_pages(st + 2, ahead);
+    if (pass == 0 && busy) {
+      // The take-th of both lists: the best over i of the lower of one's i-th
+      // and the other's (take - i)-th.
+      float other[K], bound = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < K; ++i) other[i] = __shfl_xor(tops[i], 32);
+#pragma unroll
+      for (int i = 0; i <= K; ++i) {
+        float theirs = INFINITY;
+#pragma unroll
+        for (int u = 0; u < K; ++u) theirs = u == a.take - i - 1 ? other[u] : theirs;
+        if (i <= a.take) bound = fmaxf(bound, fminf(i ? tops[i - 1] : INFINITY, theirs));
+      }
+      // A key is within a unit of its score, so what can reach the bound's
+      // lowest key lies above one unit (2^-7 of it in bf16, 2^-10 in fp16)
+      // below the bound's lowest value.
+      const float low = fmaf(-fabsf(bound), 2.4e-7f, bound) - E;
+      const float edge = low - fabsf(low) * U::kUnit - U::kSmall;
+      if (edge > floor_value) floor_value = edge;
+    }
   }
   if (!busy) return;
+  fold();
 
   const uint32_t last = key[M - 1];
   bool settled = bounded || past == 0;
-  // Exact scores of marked entries that `take` certain ones do not outrank.
-  int certain = 0;
+  // Exact scores of marked entries that `take` certain ones do not outrank:
+  // listed over the wave, then D / 16 lanes to each.
+  {
+    uint32_t* value = reinterpret_cast<uint32_t*>(&s_score[wave][0][0]);  // [entry][lane]
+    uint16_t* list = &s_id[wave][0][0];                                   // lane | entry << 6
+    uint64_t wanted = 0;
+    int certain = 0, n_list = 0;
 #pragma unroll
-  for (int i = 0; i < M; ++i) {
-    if (key[i] & 1u) {
-      if (settled && certain < a.take) {
-        const int32_t j = static_cast<int32_t>(0x7fffu - ((key[i] >> 1) & 0x7fffu));
-        const int32_t page = max(page_of(a.p, pt.seq, j), 0);
-        const uint32_t x = exact_key<T, D>(
-            q, static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D);
-        key[i] = x ? x | (key[i] & 0xfffeu) : 0u;
+    for (int i = 0; i < M; ++i) {
+      const bool marked = key[i] & 1u;
+      // Only the wave's queries: the other lanes hold leavings of its first row.
+      const bool want = marked && live && settled && certain < a.take;
+      certain += key[i] && !marked;
+      const uint64_t mask = __ballot(want);
+      if (want) {
+        list[n_list + __popcll(mask & ((uint64_t(1) << lane) - 1))] = static_cast<uint16_t>(lane | i << 6);
+        value[64 * i + lane] = key[i];
+        wanted |= uint64_t(1) << i;
       }
-    } else if (key[i]) {
-      ++certain;
+      n_list += __popcll(mask);
+      key[i] &= ~1u;
     }
-    key[i] &= ~1u;
+    wave_sync();
+    constexpr int LPR = D / 16;
+    const RotLane rl = rot_lane(lane % LPR, 0, 0);
+    for (int p0 = 0; p0 < n_list; p0 += 64 / LPR) {
+      const int p = p0 + lane / LPR;
+      const int code = list[min(p, n_list - 1)];
+      const int l = code & 63, at = 64 * (code >> 6) + l;
+      const uint32_t entry = value[at];
+      const int row = wave * 32 + (l & 31);
+      const int64_t qr = static_cast<int64_t>(pt.begin + row / group) * a.h_q + hk * group + row % group;
+      const int32_t page = max(page_of(a.p, pt.seq, static_cast<int32_t>(0x7fffu - ((entry >> 1) & 0x7fffu))), 0);
+      RawRow<T> rq, rk;
+      rq.load(static_cast<const T*>(a.q) + qr * D, rl);
+      rk.load(static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page) * a.h_kv + hk) * D, rl);
+      double t = 0.0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        t = fma(static_cast<double>(rq.element(e)), static_cast<double>(rk.element(e)), t);
+#pragma unroll
+      for (int off = 1; off < LPR; off <<= 1) t += __shfl_xor(t, off);
+      const uint32_t x = score_key<Rank<T>>(Elem<T>::round(static_cast<float>(t)));
+      if (lane % LPR == 0 && p < n_list) value[at] = x ? x | (entry & 0xfffeu) : 0u;
+    }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if ((wanted >> i) & 1) key[i] = value[64 * i + lane];
   }
   // Ranks among both lanes' entries.
   uint32_t other[M];
@@ -421,13 +523,13 @@ __global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       if (!((chosen >> i) & 1u)) continue;
-      const uint32_t id = key[i] & 0xfffeu;
+      const uint32_t me = key[i] & 0xfffeu;
       int place = 0;
 #pragma unroll
       for (int u = 0; u < M; ++u)
-        place += (((chosen >> u) & 1u) && (key[u] & 0xfffeu) > id) +
-                 (((theirs >> u) & 1u) && (other[u] & 0xfffeu) > id);
-      out[place] = static_cast<int32_t>(0x7fffu - (id >> 1));
+        place += (((chosen >> u) & 1u) && (key[u] & 0xfffeu) > me) +
+                 (((theirs >> u) & 1u) && (other[u] & 0xfffeu) > me);
+      out[place] = static_cast<int32_t>(0x7fffu - (me >> 1));
     }
     if (h == 0) {
       const int32_t o = own_entry(a.p, a.current, pt.seq, own);
@@ -442,8 +544,11 @@ __global__ void __launch_bounds__(256) tiles_kernel(GateArgs a) {
     const int row = wave * 32 + l;
     const int32_t t = pt.begin + row / group;
     const int64_t qr = static_cast<int64_t>(t) * a.h_q + hk * group + row % group;
-    exact_query<T, D, TM>(a, pt.seq, (pos0 + t) / a.p.block, hk, static_cast<const T*>(a.q) + qr * D,
-                          a.block_idx + qr * a.slots);
+    const int32_t o = (pos0 + t) / a.p.block;
+    exact_query<T, D, K>(a.p.table + static_cast<int64_t>(pt.seq) * a.p.width, a.p.pages, min(o, a.p.width),
+                         static_cast<const T*>(a.kbar) + hk * D, static_cast<int64_t>(a.h_kv) * D,
+                         static_cast<const T*>(a.q) + qr * D, a.take,
+                         own_entry(a.p, a.current, pt.seq, o), a.slots, a.block_idx + qr * a.slots);
   }
 }
 
