@@ -16,6 +16,8 @@
 // row. Entries of a column stand in no particular order; nothing depends on it.
 #include "paged_chunk.h"
 
+#include <utility>
+
 #include "paged_gate.h"
 
 namespace moba {
@@ -231,17 +233,88 @@ __device__ inline int swizzle_v(int row) {
   return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row >> 1) & 1) << 2;
 }
 
-// Eight elements of V^T for one MFMA operand: two transposing reads
-// (ds_read_b64_tr_b16), each of four keys by 16 features per 16 lanes.
-typedef short v4i16_t __attribute__((ext_vector_type(4)));
-template <typename V>
-__device__ inline V transposed(const uint16_t* p0, const uint16_t* p1) {
-  typedef __attribute__((address_space(3))) v4i16_t lds_v4i16;
-  const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p0));
-  const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p1));
-  typedef short v8i16_t __attribute__((ext_vector_type(8)));
-  const v8i16_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  return __builtin_bit_cast(V, v);
+// LDS reads of the staged rows by assembly, each block with its wait: ahead of
+// reads that it knows, the compiler waits for every load to LDS under way, the
+// next item's among them.
+__device__ inline uint32_t lds_address(const uint16_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)p));
+}
+
+__device__ inline int32_t read_word(const int32_t* p) {
+  int32_t x;
+  asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(x) : "v"(lds_address(reinterpret_cast<const uint16_t*>(p))) : "memory");
+  return x;
+}
+
+// 16 bytes at LDS address at ^ X, and STEP, 2 STEP, .. bytes behind it. The
+// exclusive or stands here so that a register holds one address, not one for
+// every X.
+template <int X, int STEP>
+__device__ inline void read_rows(uint32_t at, u32x4 (&x)[1]) {
+  uint32_t t;
+  asm volatile("v_xor_b32 %1, %3, %2\n\t"
+               "ds_read_b128 %0, %1\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(t)
+               : "v"(at), "n"(X)
+               : "memory");
+}
+template <int X, int STEP>
+__device__ inline void read_rows(uint32_t at, u32x4 (&x)[2]) {
+  uint32_t t;
+  asm volatile("v_xor_b32 %2, %4, %3\n\t"
+               "ds_read_b128 %0, %2\n\t"
+               "ds_read_b128 %1, %2 offset:%5\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(t)
+               : "v"(at), "n"(X), "n"(STEP)
+               : "memory");
+}
+template <int X, int STEP>
+__device__ inline void read_rows(uint32_t at, u32x4 (&x)[3]) {
+  uint32_t t;
+  asm volatile("v_xor_b32 %3, %5, %4\n\t"
+               "ds_read_b128 %0, %3\n\t"
+               "ds_read_b128 %1, %3 offset:%6\n\t"
+               "ds_read_b128 %2, %3 offset:%7\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(t)
+               : "v"(at), "n"(X), "n"(STEP), "n"(2 * STEP)
+               : "memory");
+}
+template <int X, int STEP>
+__device__ inline void read_rows(uint32_t at, u32x4 (&x)[4]) {
+  uint32_t t;
+  asm volatile("v_xor_b32 %4, %6, %5\n\t"
+               "ds_read_b128 %0, %4\n\t"
+               "ds_read_b128 %1, %4 offset:%7\n\t"
+               "ds_read_b128 %2, %4 offset:%8\n\t"
+               "ds_read_b128 %3, %4 offset:%9\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(t)
+               : "v"(at), "n"(X), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP)
+               : "memory");
+}
+
+// Eight elements of V^T for one MFMA operand: two transposing reads, each of
+// four keys by 16 features per 16 lanes, at a ^ X and b ^ X; for feature tiles
+// X and X + 64; AT bytes behind.
+template <int X, int AT>
+__device__ inline void read_transposed(uint32_t a, uint32_t b, u32x2 (&x)[4]) {
+  uint32_t t, u;
+  asm volatile("v_xor_b32 %4, %8, %6\n\t"
+               "v_xor_b32 %5, %8, %7\n\t"
+               "ds_read_b64_tr_b16 %0, %4 offset:%10\n\t"
+               "ds_read_b64_tr_b16 %1, %5 offset:%10\n\t"
+               "v_xor_b32 %4, %9, %6\n\t"
+               "v_xor_b32 %5, %9, %7\n\t"
+               "ds_read_b64_tr_b16 %2, %4 offset:%10\n\t"
+               "ds_read_b64_tr_b16 %3, %5 offset:%10\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(t), "=&v"(u)
+               : "v"(a), "v"(b), "n"(X), "n"(X ^ 64), "n"(AT)
+               : "memory");
 }
 
 // 16 bytes from global memory straight to LDS: lane i's to `dst` + 16 i.
@@ -274,6 +347,11 @@ __device__ inline void load_word_to_lds(const void* src, void* dst) {
       (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
 }
 
+template <int... J, typename F>
+__device__ inline void steps(std::integer_sequence<int, J...>, F&& f) {
+  (f(std::integral_constant<int, J>{}), ...);
+}
+
 // KT tiles of 32 keys cover the block. A wave holds 32 entries, one per lane
 // pair (lane, lane ^ 32):
 //   S^T[key][entry] = K . Q^T,   O^T[feature][entry] = V^T . P^T
@@ -290,8 +368,9 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   constexpr int KEYS = 32 * KT;
   constexpr int RQ = D / 8;   // 16-byte pieces per row
   constexpr int DT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[KEYS * D];
-  __shared__ __attribute__((aligned(16))) uint16_t Vs[KEYS * D];
+  // Aligned to the rows, whose bits the exclusive ors of the reads change.
+  __shared__ __attribute__((aligned(256))) uint16_t Ks[KEYS * D];
+  __shared__ __attribute__((aligned(256))) uint16_t Vs[KEYS * D];
   __shared__ int32_t s_ent[2][4][64];
   __shared__ int s_bad;  // the values hold infinities or NaN
   constexpr int LOADS = KEYS * RQ / 256;  // per thread, for the keys or the values
@@ -342,14 +421,13 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   // Rows past the sequence's end hold anything, their weights are 0. Rows past
   // the page (blocks that are no multiple of 32) read its last one.
   constexpr int ROWS = 256 / RQ;  // rows per load; the swizzles repeat every 16
-  const uint32_t row0 = tid / RQ, piece = tid % RQ;
-  const uint32_t last = a.p.block - 1;
-  auto load_rows = [&](const uint16_t* src, uint16_t* dst, uint32_t swizzled) {
+  const int row0 = tid / RQ, piece = tid % RQ;
+  const int last = a.p.block - 1;
+  auto load_rows = [&](const uint16_t* src, uint16_t* dst, int swizzled) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-      uint32_t row = u * ROWS + row0;
-      if ((u + 1) * ROWS > 32 * (KT - 1)) row = min(row, last);
-      load_to_lds(src + (row * D + swizzled), dst + (u * 256 + wave * 64) * 8);
+      const int row = (u + 1) * ROWS > 32 * (KT - 1) ? min(row0, last - u * ROWS) : row0;
+      load_to_lds(src + u * ROWS * D + (row * D + swizzled), dst + (u * 256 + wave * 64) * 8);
     }
   };
   auto load_keys = [&](const Item& d) { load_rows(d.k, Ks, 8 * (piece ^ swizzle_k<D>(row0))); };
@@ -361,20 +439,21 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
     for (int k = 0; k < D / 16; ++k) bq[k] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(q + 16 * k));
   };
 
-  // LDS addresses: of the keys' operands by K-step (tiles 32 rows apart), of
-  // the values' by feature tile (steps of 16 keys apart; the swizzle of a row
-  // depends on its place among 16).
-  const uint16_t* ka[D / 16];
+  // The compiler's wait for the queries, which it makes one for every load
+  // under way, falls here: before the values are asked for.
+  auto have_query = [&]() {
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) ka[k] = &Ks[col * D + 8 * ((2 * k + h) ^ swizzle_k<D>(col))];
-  const uint16_t *va0[DT], *va1[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int key = 4 * h + ((lane & 15) >> 2);
-    const int piece = dt * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    va0[dt] = &Vs[key * D + 8 * (piece ^ swizzle_v<D>(key)) + 4 * (lane & 1)];
-    va1[dt] = &Vs[(key + 8) * D + 8 * (piece ^ swizzle_v<D>(key + 8)) + 4 * (lane & 1)];
-  }
+    for (int k = 0; k < D / 16; ++k) asm volatile("" : "+v"(bq[k]));
+  };
+
+  // LDS addresses: of the keys' operand of K-step 0, the others by exclusive or
+  // (tiles 32 rows apart); of the values' of feature tile 0, likewise (steps of
+  // 16 keys apart: the swizzle of a row depends on its place among 16).
+  const uint32_t k_at = lds_address(&Ks[col * D + 8 * (h ^ swizzle_k<D>(col))]);
+  const int vkey = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t v_at = lds_address(&Vs[vkey * D + 8 * (vpiece ^ swizzle_v<D>(vkey)) + 4 * (lane & 1)]);
+  const uint32_t v_at8 =
+      lds_address(&Vs[(vkey + 8) * D + 8 * (vpiece ^ swizzle_v<D>(vkey + 8)) + 4 * (lane & 1)]);
 
   // One item ahead: its queries and keys are on their way from when this
   // item's first product is done, its values from when the second is. The
@@ -387,14 +466,15 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   load_entries(d, 0);
   load_entries(next, 1);
   wait_loads<0>();
-  load_query(s_ent[0][wave][lane]);
+  load_query(read_word(&s_ent[0][wave][lane]));
+  have_query();
   load_keys(d);
   load_values(d);
   for (int odd = 0;; odd ^= 1) {
     const bool more = item + stride < n_items;
     const bool work = wave * 32 < d.count;
     const bool live = wave * 32 + col < d.count;
-    const int32_t ent = s_ent[odd][wave][lane];
+    const int32_t ent = read_word(&s_ent[odd][wave][lane]);
     const int lim = live ? min(d.key_lim - 1, d.pos0 + ent / a.slots / a.h_q) : -1;  // last key seen
     wait_loads<LOADS>();  // all but the values
     meet();
@@ -403,19 +483,21 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
     if (work) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) s[kt] = floatx16_t{};
+      auto step = [&](auto kc) {
+        constexpr int k = decltype(kc)::value;
+        u32x4 x[KT];
+        read_rows<32 * k, 32 * D * 2>(k_at, x);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-          s[kt] = M::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(ka[k] + kt * 32 * D)), bq[k], s[kt]);
+        for (int kt = 0; kt < KT; ++kt) s[kt] = M::mma(__builtin_bit_cast(V8, x[kt]), bq[k], s[kt]);
+      };
+      steps(std::make_integer_sequence<int, D / 16>{}, step);
     }
     meet();  // every wave is done with the keys
     Item after = next;
     if (more) {
       after = describe(min(item + 2 * stride, n_items - 1));
-      const int32_t next_ent = s_ent[odd ^ 1][wave][lane];
+      load_query(read_word(&s_ent[odd ^ 1][wave][lane]));
       load_entries(after, odd);
-      load_query(next_ent);
       load_keys(next);
     }
     const bool whole = __all(!live || lim == KEYS - 1);
@@ -485,48 +567,58 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
         meet();
       }
     }
+    // Two feature tiles at a time, rounded and kept until the queries are in.
+    typedef typename M::scalar S4 __attribute__((ext_vector_type(4)));
+    S4 rows[DT][4];
     if (work) {
-      // Value operand of features 32 dt + [0, 32) and keys 16 j + [0, 16).
-      auto values = [&](int j, int dt) { return transposed<V8>(va0[dt] + j * 16 * D, va1[dt] + j * 16 * D); };
-      floatx16_t o[DT];
+      auto half = [&](auto pc) {
+        constexpr int dt = 2 * decltype(pc)::value;
+        floatx16_t o[2] = {floatx16_t{}, floatx16_t{}};
+        // Features 32 dt + [0, 64), keys 16 j + [0, 16).
+        auto step = [&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          u32x2 x[4];
+          read_transposed<64 * dt, j * 16 * D * 2>(v_at, v_at8, x);
+          o[0] = M::mma(__builtin_bit_cast(V8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]}), bp[j], o[0]);
+          o[1] = M::mma(__builtin_bit_cast(V8, u32x4{x[2][0], x[2][1], x[3][0], x[3][1]}), bp[j], o[1]);
+        };
+        steps(std::make_integer_sequence<int, KEYS / 16>{}, step);
+        if (bad) {
+          // What the queries see of the values that were taken out.
+          for (int key = 0; key < d.key_lim; ++key) {
+            const uint16_t* row = d.v + key * D + 32 * dt + 4 * h;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = floatx16_t{};
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int j = 0; j < KEYS / 16; ++j)
+              for (int q4 = 0; q4 < 4; ++q4) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(row + t * 32 + 8 * q4);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = M::mma(values(j, dt), bp[j], o[dt]);
-      if (bad) {
-        // What the queries see of the values that were taken out.
-        for (int key = 0; key < d.key_lim; ++key) {
-          const uint16_t* row = d.v + key * D + 4 * h;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              const u32x2 x = *reinterpret_cast<const u32x2*>(row + dt * 32 + 8 * q4);
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint16_t bits = static_cast<uint16_t>(x[w >> 1] >> (16 * (w & 1)));
-                if ((bits & M::kInf) == M::kInf && key <= lim)
-                  o[dt][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
+                for (int w = 0; w < 4; ++w) {
+                  const uint16_t bits = static_cast<uint16_t>(x[w >> 1] >> (16 * (w & 1)));
+                  if ((bits & M::kInf) == M::kInf && key <= lim)
+                    o[t][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
+                }
               }
-            }
-        }
-      }
-      if (live) {
-        if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * static_cast<int64_t>(ent)) = make_float2(m, l);
-        uint16_t* dst = static_cast<uint16_t*>(a.part_acc) + static_cast<int64_t>(ent) * D + 4 * h;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            typedef typename M::scalar S4 __attribute__((ext_vector_type(4)));
-            S4 x;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) x[w] = static_cast<typename M::scalar>(o[dt][4 * q4 + w]);
-            *reinterpret_cast<u32x2*>(dst + dt * 32 + 8 * q4) = __builtin_bit_cast(u32x2, x);
           }
-      }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) rows[dt + t][q4][w] = static_cast<typename M::scalar>(o[t][4 * q4 + w]);
+      };
+      steps(std::make_integer_sequence<int, DT / 2>{}, half);
+    }
+    have_query();
+    if (live && work) {
+      if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * static_cast<int64_t>(ent)) = make_float2(m, l);
+      uint16_t* dst = static_cast<uint16_t*>(a.part_acc) + static_cast<int64_t>(ent) * D + 4 * h;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<u32x2*>(dst + dt * 32 + 8 * q4) = __builtin_bit_cast(u32x2, rows[dt][q4]);
     }
     meet();  // every wave is done with the values
     if (!more) break;
