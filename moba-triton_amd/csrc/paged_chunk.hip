@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kSortThreads) column_place_kernel(ChunkArgs a)
       if (blk[u] >= 0)
         a.entries[atomicAdd(&cursor[blk[u]], 1)] = e[u];
       else if (i0 + kSortThreads * u < n)
-        *reinterpret_cast<float2*>(a.part_ml + 2 * static_cast<int64_t>(e[u])) = make_float2(-INFINITY, 0.f);
+        a.part_ml[e[u]] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
     }
   }
 }
@@ -347,6 +347,63 @@ __device__ inline void load_word_to_lds(const void* src, void* dst) {
       (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
 }
 
+// A half of a partial row, 64 features, as whole numbers of 16 bits and a unit
+// that is 1/32700 of the half's largest magnitude: half the bytes of float32 at
+// an error below 2^-16 of that largest, where rounding to bf16 is off by up to
+// 2^-9 of every element (a query's 8 partial rows then added as much error as
+// the rounding of the result does, at no less traffic).
+// A half with infinities or NaN has a negative unit and codes for them.
+constexpr int kCodes = 32700, kInfCode = 32767, kNanCode = 0x8000;
+constexpr float kLeast = 0x1p-110f;  // largest magnitudes below it count as it
+
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one is
+
+__device__ inline uint32_t special_code(float x, uint32_t code) {
+  if (x != x) return kNanCode;
+  return fabsf(x) < INFINITY ? code : (x > 0.f ? kInfCode : -kInfCode) & 0xffffu;
+}
+
+// o[t][i], 32 features of the lane; lane ^ 32 has the others.
+__device__ inline float half_codes(const floatx16_t (&o)[2], u32x2 (&code)[2][4]) {
+  float top = 0.f;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = larger(top, fabsf(o[t][i]));
+  top = larger(top, __shfl_xor(top, 32));
+  const bool strange = !(top < INFINITY);
+  const bool any = __any(strange);
+  if (any) {
+    float finite = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) finite = fmaxf(finite, fabsf(o[t][i]) < INFINITY ? fabsf(o[t][i]) : 0.f);
+    top = fmaxf(finite, __shfl_xor(finite, 32));
+  }
+  top = fmaxf(top, kLeast);
+  // The conversion multiplies by 32767 and rounds to the nearest.
+  const float per = (kCodes / 32767.f) * __builtin_amdgcn_rcpf(top);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const float x = o[t][4 * q4 + 2 * w], y = o[t][4 * q4 + 2 * w + 1];
+        uint32_t c = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(x * per, y * per));
+        if (any) c = special_code(x, c & 0xffffu) | (special_code(y, c >> 16) << 16);
+        code[t][q4][w] = c;
+      }
+  const float unit = top * (1.f / kCodes);
+  return strange ? -unit : unit;
+}
+
+__device__ inline float of_special(int code) {
+  if (code > -kInfCode && code < kInfCode) return static_cast<float>(code);
+  return code < -kInfCode ? NAN : code > 0 ? INFINITY : -INFINITY;
+}
+
 template <int... J, typename F>
 __device__ inline void steps(std::integer_sequence<int, J...>, F&& f) {
   (f(std::integral_constant<int, J>{}), ...);
@@ -359,8 +416,7 @@ __device__ inline void steps(std::integer_sequence<int, J...>, F&& f) {
 // second's operand (its keys in the order 8 (u / 4) + 4 h + u % 4 of lane half
 // h, which the values' reads follow). P is rounded to the type for the
 // product, as the framework's forward does; m and l stay in float32. Partial
-// rows are rounded to the type once: their weighted mean moves by at most half
-// a step of the weighted mean of |v|.
+// rows leave in halves of 64 features, as codes (Half).
 template <typename T, int D, int KT>
 __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   using M = Unit<T>;
@@ -567,12 +623,12 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
         meet();
       }
     }
-    // Two feature tiles at a time, rounded and kept until the queries are in.
-    typedef typename M::scalar S4 __attribute__((ext_vector_type(4)));
-    S4 rows[DT][4];
+    // Two feature tiles at a time, encoded and kept until the queries are in.
+    u32x2 rows[DT / 2][2][4];
+    float units[2] = {0.f, 0.f};
     if (work) {
       auto half = [&](auto pc) {
-        constexpr int dt = 2 * decltype(pc)::value;
+        constexpr int half_row = decltype(pc)::value, dt = 2 * half_row;
         floatx16_t o[2] = {floatx16_t{}, floatx16_t{}};
         // Features 32 dt + [0, 64), keys 16 j + [0, 16).
         auto step = [&](auto jc) {
@@ -601,24 +657,19 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
               }
           }
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) rows[dt + t][q4][w] = static_cast<typename M::scalar>(o[t][4 * q4 + w]);
+        units[half_row] = half_codes(o, rows[half_row]);
       };
       steps(std::make_integer_sequence<int, DT / 2>{}, half);
     }
     have_query();
     if (live && work) {
-      if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * static_cast<int64_t>(ent)) = make_float2(m, l);
+      if (h == 0) a.part_ml[ent] = make_float4(m, l, units[0], units[1]);
       uint16_t* dst = static_cast<uint16_t*>(a.part_acc) + static_cast<int64_t>(ent) * D + 4 * h;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<u32x2*>(dst + dt * 32 + 8 * q4) = __builtin_bit_cast(u32x2, rows[dt][q4]);
+          *reinterpret_cast<u32x2*>(dst + dt * 32 + 8 * q4) = rows[dt / 2][dt % 2][q4];
     }
     meet();  // every wave is done with the values
     if (!more) break;
@@ -638,7 +689,7 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
   const int c = threadIdx.x % LPR;
   for (int hd = threadIdx.x / LPR; hd < a.h_q; hd += blockDim.x / LPR) {
     const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * a.h_q + hd) * a.slots;
-    const float* ml = a.part_ml + 2 * e0;
+    const float4* ml = a.part_ml + e0;
     const u32x4* acc = static_cast<const u32x4*>(a.part_acc) + e0 * LPR + c;
     // Eight slots in flight. Those that were not written (m = -inf) hold
     // anything: they count as zeros.
@@ -646,12 +697,12 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.f;
     for (int j0 = 0; j0 < a.slots; j0 += 8) {
-      float2 x[8];
+      float4 x[8];
       u32x4 raw[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int j = min(j0 + u, a.slots - 1);
-        x[u] = *reinterpret_cast<const float2*>(ml + 2 * j);
+        x[u] = ml[j];
         raw[u] = acc[j * LPR];
       }
       float m = top;
@@ -665,16 +716,29 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
       total *= old;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] *= old;
+      auto add = [&](auto with) {
+        constexpr bool kSpecial = decltype(with)::value;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const bool in = x[u].x != -INFINITY;
-        const float w = __builtin_amdgcn_exp2f(x[u].x - z);
-        total = fmaf(in ? x[u].y : 0.f, w, total);
-        const u32x4 r = in ? raw[u] : u32x4{0, 0, 0, 0};
-        const T* v = reinterpret_cast<const T*>(&r);
+        for (int u = 0; u < 8; ++u) {
+          const bool in = x[u].x != -INFINITY;
+          const float w = __builtin_amdgcn_exp2f(x[u].x - z);
+          total = fmaf(in ? x[u].y : 0.f, w, total);
+          const float wu = in ? fabsf(c < 8 ? x[u].z : x[u].w) * w : 0.f;
+          const bool mine = kSpecial && in && (c < 8 ? x[u].z : x[u].w) < 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(Elem<T>::load(v, e), w, o[e]);
-      }
+          for (int e = 0; e < 8; ++e) {
+            const int code = static_cast<int16_t>(raw[u][e >> 1] >> (16 * (e & 1)));
+            o[e] = fmaf(mine ? of_special(code) : static_cast<float>(code), wu, o[e]);
+          }
+        }
+      };
+      bool special = false;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) special |= x[u].x != -INFINITY && fminf(x[u].z, x[u].w) < 0.f;
+      if (__any(special))
+        add(std::true_type{});
+      else
+        add(std::false_type{});
       top = m;
     }
     const int64_t row = static_cast<int64_t>(tok) * a.h_q + hd;
@@ -719,8 +783,8 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   pl.table = take(sizeof(int32_t) * static_cast<size_t>(pl.parts * row));
   pl.items = take(sizeof(int4) * static_cast<size_t>(pl.max_items));
   pl.entries = take(sizeof(int32_t) * static_cast<size_t>(entries));
-  pl.ml = take(sizeof(float) * 2 * static_cast<size_t>(entries));
-  pl.acc = take(2 * static_cast<size_t>(entries * c.head_dim));
+  pl.ml = take(sizeof(float4) * static_cast<size_t>(entries));
+  pl.acc = take(sizeof(int16_t) * static_cast<size_t>(entries * c.head_dim));
   pl.total = o;
   return pl;
 }
@@ -740,7 +804,7 @@ int chunk_attend(const moba_paged& c, const Paged& p, void* workspace, hipStream
   a.table = reinterpret_cast<int32_t*>(ws + pl.table);
   a.items = reinterpret_cast<int4*>(ws + pl.items);
   a.entries = reinterpret_cast<int32_t*>(ws + pl.entries);
-  a.part_ml = reinterpret_cast<float*>(ws + pl.ml);
+  a.part_ml = reinterpret_cast<float4*>(ws + pl.ml);
   a.part_acc = ws + pl.acc;
   a.h_q = static_cast<int>(c.h_q);
   a.h_kv = static_cast<int>(c.h_kv);
