@@ -19,6 +19,7 @@
 #include <utility>
 
 #include "paged_gate.h"
+#include "paged_lds.h"
 
 namespace moba {
 
@@ -27,8 +28,6 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Unit;
 template <> struct Unit<bf16_t> {
@@ -223,128 +222,11 @@ __global__ void __launch_bounds__(kSortThreads) column_place_kernel(ChunkArgs a)
   }
 }
 
-// 16-byte pieces of a row stand in LDS at piece ^ swizzle(row), so that the 16
-// rows a wave's lanes read together (keys), or the four rows of a transposing
-// read (values), fall into different banks.
-template <int D>
-__device__ inline int swizzle_k(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+// The values' pieces stand so that the four rows of a transposing read fall
+// into different banks.
 template <int D>
 __device__ inline int swizzle_v(int row) {
   return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row >> 1) & 1) << 2;
-}
-
-// LDS reads of the staged rows by assembly, each block with its wait: ahead of
-// reads that it knows, the compiler waits for every load to LDS under way, the
-// next item's among them.
-__device__ inline uint32_t lds_address(const uint16_t* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)p));
-}
-
-__device__ inline int32_t read_word(const int32_t* p) {
-  int32_t x;
-  asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)"
-               : "=&v"(x) : "v"(lds_address(reinterpret_cast<const uint16_t*>(p))) : "memory");
-  return x;
-}
-
-// 16 bytes at LDS address at ^ X, and STEP, 2 STEP, .. bytes behind it. The
-// exclusive or stands here so that a register holds one address, not one for
-// every X.
-template <int X, int STEP>
-__device__ inline void read_rows(uint32_t at, u32x4 (&x)[1]) {
-  uint32_t t;
-  asm volatile("v_xor_b32 %1, %3, %2\n\t"
-               "ds_read_b128 %0, %1\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(x[0]), "=&v"(t)
-               : "v"(at), "n"(X)
-               : "memory");
-}
-template <int X, int STEP>
-__device__ inline void read_rows(uint32_t at, u32x4 (&x)[2]) {
-  uint32_t t;
-  asm volatile("v_xor_b32 %2, %4, %3\n\t"
-               "ds_read_b128 %0, %2\n\t"
-               "ds_read_b128 %1, %2 offset:%5\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(t)
-               : "v"(at), "n"(X), "n"(STEP)
-               : "memory");
-}
-template <int X, int STEP>
-__device__ inline void read_rows(uint32_t at, u32x4 (&x)[3]) {
-  uint32_t t;
-  asm volatile("v_xor_b32 %3, %5, %4\n\t"
-               "ds_read_b128 %0, %3\n\t"
-               "ds_read_b128 %1, %3 offset:%6\n\t"
-               "ds_read_b128 %2, %3 offset:%7\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(t)
-               : "v"(at), "n"(X), "n"(STEP), "n"(2 * STEP)
-               : "memory");
-}
-template <int X, int STEP>
-__device__ inline void read_rows(uint32_t at, u32x4 (&x)[4]) {
-  uint32_t t;
-  asm volatile("v_xor_b32 %4, %6, %5\n\t"
-               "ds_read_b128 %0, %4\n\t"
-               "ds_read_b128 %1, %4 offset:%7\n\t"
-               "ds_read_b128 %2, %4 offset:%8\n\t"
-               "ds_read_b128 %3, %4 offset:%9\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(t)
-               : "v"(at), "n"(X), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP)
-               : "memory");
-}
-
-// Eight elements of V^T for one MFMA operand: two transposing reads, each of
-// four keys by 16 features per 16 lanes, at a ^ X and b ^ X; for feature tiles
-// X and X + 64; AT bytes behind.
-template <int X, int AT>
-__device__ inline void read_transposed(uint32_t a, uint32_t b, u32x2 (&x)[4]) {
-  uint32_t t, u;
-  asm volatile("v_xor_b32 %4, %8, %6\n\t"
-               "v_xor_b32 %5, %8, %7\n\t"
-               "ds_read_b64_tr_b16 %0, %4 offset:%10\n\t"
-               "ds_read_b64_tr_b16 %1, %5 offset:%10\n\t"
-               "v_xor_b32 %4, %9, %6\n\t"
-               "v_xor_b32 %5, %9, %7\n\t"
-               "ds_read_b64_tr_b16 %2, %4 offset:%10\n\t"
-               "ds_read_b64_tr_b16 %3, %5 offset:%10\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(t), "=&v"(u)
-               : "v"(a), "v"(b), "n"(X), "n"(X ^ 64), "n"(AT)
-               : "memory");
-}
-
-// 16 bytes from global memory straight to LDS: lane i's to `dst` + 16 i.
-__device__ inline void load_to_lds(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds(
-      reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
-      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
-
-// Waits until at most N of the wave's vector memory operations are under way
-// (they end in order). Loads to LDS count as such: a barrier alone does not
-// wait for them.
-template <int N>
-__device__ inline void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// A barrier that waits for no vector memory (__syncthreads waits for every
-// load to LDS under way): each wave waits for its own before.
-__device__ inline void meet() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// 4 bytes each: lane i's to `dst` + 4 i.
-__device__ inline void load_word_to_lds(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds(
-      reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
-      (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
 }
 
 // A half of a partial row, 64 features, as whole numbers of 16 bits and a unit
@@ -402,11 +284,6 @@ __device__ inline float half_codes(const floatx16_t (&o)[2], u32x2 (&code)[2][4]
 __device__ inline float of_special(int code) {
   if (code > -kInfCode && code < kInfCode) return static_cast<float>(code);
   return code < -kInfCode ? NAN : code > 0 ? INFINITY : -INFINITY;
-}
-
-template <int... J, typename F>
-__device__ inline void steps(std::integer_sequence<int, J...>, F&& f) {
-  (f(std::integral_constant<int, J>{}), ...);
 }
 
 // KT tiles of 32 keys cover the block. A wave holds 32 entries, one per lane
@@ -486,7 +363,7 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
       load_to_lds(src + u * ROWS * D + (row * D + swizzled), dst + (u * 256 + wave * 64) * 8);
     }
   };
-  auto load_keys = [&](const Item& d) { load_rows(d.k, Ks, 8 * (piece ^ swizzle_k<D>(row0))); };
+  auto load_keys = [&](const Item& d) { load_rows(d.k, Ks, 8 * (piece ^ swizzle_rows<D>(row0))); };
   auto load_values = [&](const Item& d) { load_rows(d.v, Vs, 8 * (piece ^ swizzle_v<D>(row0))); };
   V8 bq[D / 16];
   auto load_query = [&](int32_t ent) {
@@ -505,7 +382,7 @@ __global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
   // LDS addresses: of the keys' operand of K-step 0, the others by exclusive or
   // (tiles 32 rows apart); of the values' of feature tile 0, likewise (steps of
   // 16 keys apart: the swizzle of a row depends on its place among 16).
-  const uint32_t k_at = lds_address(&Ks[col * D + 8 * (h ^ swizzle_k<D>(col))]);
+  const uint32_t k_at = lds_address(&Ks[col * D + 8 * (h ^ swizzle_rows<D>(col))]);
   const int vkey = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const uint32_t v_at = lds_address(&Vs[vkey * D + 8 * (vpiece ^ swizzle_v<D>(vkey)) + 4 * (lane & 1)]);
   const uint32_t v_at8 =

@@ -10,6 +10,7 @@
 //   scores in float64, over the whole chip, then one wave per query.
 // * tiles_kernel: 16-bit types, many queries (below).
 #include "paged_gate.h"
+#include "paged_lds.h"
 
 #include <type_traits>
 
@@ -22,7 +23,6 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Scores of one token's query heads of one kv head against a run of its past
 // blocks: a block's representative belongs to D / 16 lanes, which hold it in
@@ -65,23 +65,47 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(GateArgs a) {
     RawRow<T> raw[H];
 #pragma unroll
     for (int u = 0; u < H; ++u) raw[u].load(q + min(h0 + u, group - 1) * D, rl);
+    // Element i H + u is block i's and head u's share of this lane. The sums over
+    // the lanes halve a lane's elements with every exchange, as long as it has
+    // several: 7 exchanges at D = 128, not 24.
+    constexpr int N = kScoreRows * H;
+    double t[N] = {};
 #pragma unroll
-    for (int u = 0; u < H; ++u) {
-      double t[kScoreRows] = {};
+    for (int u = 0; u < H; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const double x = static_cast<double>(raw[u].element(e));
 #pragma unroll
-        for (int i = 0; i < kScoreRows; ++i) t[i] = fma(x, kd[i][e], t[i]);
+        for (int i = 0; i < kScoreRows; ++i) t[i * H + u] = fma(x, kd[i][e], t[i * H + u]);
       }
+    int first = 0;  // the lane's elements are first, first + 1, ..
 #pragma unroll
-      for (int i = 0; i < kScoreRows; ++i) {
+    for (int off = 1; off < LPR; off <<= 1) {
+      const int left = N / (2 * off);
+      if (left > 0) {
+        const bool upper = lane & off;
+        first += upper ? left : 0;
 #pragma unroll
-        for (int off = 1; off < LPR; off <<= 1) t[i] += __shfl_xor(t[i], off);
+        for (int e = 0; e < left; ++e) {
+          const double give = upper ? t[e] : t[e + left];
+          t[e] = (upper ? t[e + left] : t[e]) + __shfl_xor(give, off);
+        }
+      } else {
+        t[0] += __shfl_xor(t[0], off);
+      }
+    }
+    if (lane < N) {
+#pragma unroll
+      for (int e = 0; e < (N / LPR > 0 ? N / LPR : 1); ++e) {
+        const int i = (first + e) / H, u = (first + e) % H;
         const int32_t j = j0 + i * G + g;
-        if (lane == 0 && j < past && h0 + u < group)
+        if (j < past && h0 + u < group) {
+          int32_t pg = page[0];
+#pragma unroll
+          for (int x = 1; x < kScoreRows; ++x) pg = i == x ? page[x] : pg;
           a.keys[(row0 + h0 + u) * a.p.width + j] =
-              page[i] < 0 ? 0u : score_key<Rank<T>>(Elem<T>::round(static_cast<float>(t[i])));
+              pg < 0 ? 0u : score_key<Rank<T>>(Elem<T>::round(static_cast<float>(t[e])));
+        }
       }
     }
   }
@@ -261,9 +285,10 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
   constexpr int RQ = D / 8;     // 16-byte pieces per row
   constexpr int ROWS = 64;      // representatives per stage
   constexpr int KS = D / 16;
-  __shared__ __attribute__((aligned(16))) uint16_t rows[2][ROWS * D];
+  // Aligned to the rows, whose bits the exclusive ors of the reads change.
+  __shared__ __attribute__((aligned(512))) uint16_t rows[2][ROWS * D];
   __shared__ int32_t s_page[2][ROWS];
-  __shared__ uint64_t s_valid[4];
+  __shared__ int32_t s_valid[4][2];
   constexpr int kHeld = M > kBuffer ? M : kBuffer;
   __shared__ float s_score[4][kHeld][64];
   __shared__ uint16_t s_id[4][kHeld][64];
@@ -308,28 +333,32 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
   const bool bounded = qn * kn < 3e38f && E < 3e38f;  // false for infinities and NaN
 
   // Pages of stage st, by wave 0: to LDS, with a bit for each that is one.
-  auto page_at = [&](int st) {
-    const int32_t j = st * ROWS + lane;
-    return j < horizon ? page_of(a.p, pt.seq, j) : -1;
-  };
+  const int32_t* pages = a.p.table + static_cast<int64_t>(pt.seq) * a.p.width;
+  auto page_at = [&](int st) { return pages[min(st * ROWS + lane, horizon - 1)]; };
   auto put_pages = [&](int st, int32_t page) {
-    const uint64_t ok = __ballot(page >= 0);
-    s_page[st & 1][lane] = max(page, 0);
-    if (lane == 0) s_valid[st & 3] = ok;
+    const bool is = st * ROWS + lane < horizon && page >= 0 && page < a.p.pages;
+    const uint64_t ok = __ballot(is);
+    s_page[st & 1][lane] = is ? page : 0;
+    if (lane == 0) {
+      s_valid[st & 3][0] = static_cast<int32_t>(ok);
+      s_valid[st & 3][1] = static_cast<int32_t>(ok >> 32);
+    }
   };
   auto stage = [&](int st) {
+    int32_t page[ROWS * RQ / 256];
+#pragma unroll
+    for (int u = 0; u < ROWS * RQ / 256; ++u) page[u] = s_page[st & 1][(u * 256 + tid) / RQ];
 #pragma unroll
     for (int u = 0; u < ROWS * RQ / 256; ++u) {
       const int i = u * 256 + tid, row = i / RQ, piece = i % RQ;
-      const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
-      const T* src = static_cast<const T*>(a.kbar) +
-                     (static_cast<int64_t>(s_page[st & 1][row]) * a.h_kv + hk) * D + 8 * (piece ^ swz);
-      __builtin_amdgcn_global_load_lds(
-          reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
-          (__attribute__((address_space(3))) void*)&rows[st & 1][(u * 256 + wave * 64) * 8], 16, 0, 0);
+      const T* src = static_cast<const T*>(a.kbar) + (static_cast<int64_t>(page[u]) * a.h_kv + hk) * D +
+                     8 * (piece ^ swizzle_rows<D>(row));
+      load_to_lds(src, &rows[st & 1][(u * 256 + wave * 64) * 8]);
     }
   };
 
+  // Representatives lane & 31 and 32 more: feature step 0 of the first stage.
+  const uint32_t k_at0 = lds_address(&rows[0][(lane & 31) * D + 8 * (h ^ swizzle_rows<D>(lane & 31))]);
   uint32_t key[M];
 #pragma unroll
   for (int i = 0; i < M; ++i) key[i] = 0;
@@ -364,29 +393,30 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
     __syncthreads();
     stage(0);
     for (int st = 0; st < stages; ++st) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+      wait_loads<0>();
+      meet();
       int32_t ahead = -1;
       if (wave == 0 && st + 2 < stages) ahead = page_at(st + 2);
       if (st + 1 < stages) stage(st + 1);
       if (busy) {
-        const uint64_t valid = s_valid[st & 3];
+        const uint32_t valid[2] = {static_cast<uint32_t>(read_word(&s_valid[st & 3][0])),
+                                   static_cast<uint32_t>(read_word(&s_valid[st & 3][1]))};
         floatx16_t s[2] = {floatx16_t{}, floatx16_t{}};
+        const uint32_t k_at = k_at0 + (st & 1) * ROWS * D * 2;
+        auto step = [&](auto kc) {
+          constexpr int k = decltype(kc)::value;
+          u32x4 x[4];
+          read_row_pairs<64 * k, 32 * D * 2>(k_at, x);
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int row = half * 32 + (lane & 31);
-            const int swz = D == 64 ? (row >> 1) & 7 : row & 15;
-            s[half] = U::mma(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(
-                                                        &rows[st & 1][row * D + 8 * ((2 * k + h) ^ swz)])),
-                             bq[k], s[half]);
-          }
+          for (int u = 0; u < 4; ++u)
+            s[u & 1] = U::mma(__builtin_bit_cast(V8, x[u]), bq[2 * k + (u >> 1)], s[u & 1]);
+        };
+        steps(std::make_integer_sequence<int, KS / 2>{}, step);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int32_t j0 = st * ROWS + half * 32;
           if (j0 >= horizon) continue;
-          const uint32_t ok = static_cast<uint32_t>(valid >> (32 * half));
+          const uint32_t ok = valid[half];
           if (j0 + 32 > sure || ok != 0xffffffffu) {  // some blocks are not for every query
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
@@ -405,12 +435,12 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
             if (__any(held > kBuffer - 16)) fold();
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
+              // Written whether it counts or not: about half of these tests
+              // hold for some lane.
               const float x = s[half][v];
-              if (fmaf(fabsf(x), 2.4e-7f, x) + E > floor_value) {
-                score[64 * held] = x;
-                id[64 * held] = static_cast<uint16_t>(j0 + 8 * (v >> 2) + 4 * h + (v & 3));
-                ++held;
-              }
+              score[64 * held] = x;
+              id[64 * held] = static_cast<uint16_t>(j0 + 8 * (v >> 2) + 4 * h + (v & 3));
+              held += fmaf(fabsf(x), 2.4e-7f, x) + E > floor_value ? 1 : 0;
             }
           }
         }
@@ -516,20 +546,23 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
   const uint32_t out_of = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), 32)));
   if (out_of && (n < a.take || lowest < (out_of & ~1u))) settled = false;
 
-  // Places in the order of the ids: larger (0x7fff - id) first.
+  // Places in the order of the ids: larger (0x7fff - id) first, 0 for entries
+  // that are not chosen (ids are below 0x7fff).
   int32_t* out = a.block_idx + qrow * a.slots;
   const uint64_t theirs = __shfl_xor(static_cast<unsigned long long>(chosen), 32);
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    key[i] = (chosen >> i) & 1u ? key[i] & 0xfffeu : 0u;
+    other[i] = (theirs >> i) & 1u ? other[i] & 0xfffeu : 0u;
+  }
   if (settled && live) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      if (!((chosen >> i) & 1u)) continue;
-      const uint32_t me = key[i] & 0xfffeu;
+      if (!key[i]) continue;
       int place = 0;
 #pragma unroll
-      for (int u = 0; u < M; ++u)
-        place += (((chosen >> u) & 1u) && (key[u] & 0xfffeu) > me) +
-                 (((theirs >> u) & 1u) && (other[u] & 0xfffeu) > me);
-      out[place] = static_cast<int32_t>(0x7fffu - (me >> 1));
+      for (int u = 0; u < M; ++u) place += (key[u] > key[i]) + (other[u] > key[i]);
+      out[place] = static_cast<int32_t>(0x7fffu - (key[i] >> 1));
     }
     if (h == 0) {
       const int32_t o = own_entry(a.p, a.current, pt.seq, own);
