@@ -243,9 +243,13 @@ PagedPlan plan_of(const moba_paged& c) {
   PagedPlan pl;
   const int64_t rows = c.tokens * c.h_q;
   const int64_t units = c.slots * cdiv(c.block_size, run_keys(c.head_dim, static_cast<int>(c.dtype)));
-  // Few rows: wide workgroups, and several of them per row.
-  pl.waves = rows < 256 && units > 4 ? 16 : 4;
-  const int64_t splits = cdiv(512, rows * pl.waves / 4);
+  // Few rows: wide workgroups, and several of them per row. With the choice of
+  // the blocks, 32 heads of 128 over 32k keys: 256 rows by 16 waves 36 us, by 4
+  // waves 39; 512 rows by 16 waves 68 us, by 4 waves 63, as two workgroups per
+  // row (87 as one); 64 rows of 64k keys in 16 splits of 4 waves 25, in 4 of 16
+  // waves 23.
+  pl.waves = rows <= 256 && units > 4 ? 16 : 4;
+  const int64_t splits = cdiv(1024, rows * pl.waves / 4);
   const int64_t most = cdiv(units, pl.waves);
   pl.splits = splits < most ? splits : most;
   const size_t parts = pl.splits > 1 ? static_cast<size_t>(rows * pl.splits) : 0;

@@ -635,9 +635,19 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 }  // namespace
 
+// Block by block pays where an entry's block is on average another's too, and
+// where the entries' keys and values, which rows read one by one, outweigh the
+// launches. bf16, 32 and 8 heads of 128, 9 blocks of 128 per query, block by
+// block and row by row: 32 sequences of 256 blocks, 4 new tokens each (0.6
+// entries per block) 352 and 315 us, 8 each (1.1) 553 and 586, 16 each 772 and
+// 1130; one of 512 blocks, 8 tokens 48 and 27, 64 tokens (1.2 GB) 79 and 148. 8
+// heads of 64, 5 blocks of 64: 8 of 64 blocks, 64 tokens each (335 MB) 47 and 32.
+constexpr int64_t kColumnBytes = int64_t(1) << 29;
 bool chunk_takes(const moba_paged& c) {
+  const int64_t entries = c.tokens * c.h_q * c.slots;
   return c.dtype != MOBA_FP32 && (c.head_dim == 64 || c.head_dim == 128) && c.block_size <= 128 &&
-         c.table_width <= 15360 && c.h_kv <= 65535 && c.tokens >= 4 * c.seqs;
+         c.table_width <= 15360 && c.h_kv <= 65535 && entries >= c.seqs * c.h_kv * c.table_width &&
+         entries * c.block_size * c.head_dim * 4 >= kColumnBytes;
 }
 
 ChunkPlan chunk_plan(const moba_paged& c) {
@@ -646,9 +656,12 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   // Partial rows of at most 2^29 bytes at a time.
   pl.slice = (int64_t(1) << 29) / (per_token * c.head_dim * 2);
   pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
-  // Parts of 256 tokens (64: the scan over 32 parts of 2048 tokens took 22 us,
-  // over 8 parts 9), more where the count table would pass 2^22 entries.
-  pl.part = 256;
+  // Parts of 64 tokens: more workgroups count and place, and the scan walks more
+  // parts (4 x 512 tokens, 4 kv heads: the attention 157 us, in parts of 256
+  // 189; 2048 tokens, 8 kv heads: 255 and 256). Longer ones where a slice has
+  // more than 64 of them or the count table would pass 2^22 entries.
+  pl.part = 64;
+  while (pl.slice / pl.part > 64) pl.part *= 2;
   const int64_t row = c.h_kv * c.table_width;
   while (pl.part < pl.slice && (pl.slice / pl.part + c.seqs) * row > (int64_t(1) << 22)) pl.part *= 2;
   pl.parts = cdiv(pl.slice, pl.part) + c.seqs;

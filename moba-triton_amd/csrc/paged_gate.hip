@@ -592,9 +592,16 @@ __global__ void __launch_bounds__(64) nobody_kernel(GateArgs a) {
   for (int i = threadIdx.x; i < a.h_q * a.slots; i += 64) out[i] = -1;
 }
 
+// The tiles from kTileRows query rows on, where sequences have several tokens (a
+// tile holds one sequence's). bf16, 32 and 8 heads of 128, tiles and score +
+// select: 32 sequences of 256 blocks, 4 new tokens each (4096 rows) 36 and 32
+// us, 8 each 37 and 58; 4 of 512 blocks, 32 tokens each (4096 rows) 47 and 58;
+// one of 512 blocks, 64 tokens (2048 rows) 46 and 32. 8 heads of 64, 8
+// sequences of 64 blocks, 64 tokens each (4096 rows) 21 and 31, 8 each 21 and 16.
+constexpr int64_t kTileRows = 4096;
 bool tiles_take(const moba_paged& c) {
   return c.dtype != MOBA_FP32 && c.take > 0 && c.table_width < (1 << 15) && c.h_q / c.h_kv <= 128 &&
-         c.h_kv <= 65535 && c.tokens >= 4 * c.seqs;
+         c.h_kv <= 65535 && c.tokens >= 4 * c.seqs && c.tokens * c.h_q >= kTileRows;
 }
 
 int64_t score_slice(const moba_paged& c) {

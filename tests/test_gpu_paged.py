@@ -14,7 +14,7 @@ from moba.kernels.paged import (PagedKV, append_tokens, copy_pages, paged_attent
                                 paged_gate_select)
 from moba.kernels.pooling import pool_blocks
 from moba.kernels.rotary import norm_rotate
-from paged_util import (Paged, attend64, cu_of, forward_bound, norm_rotate64, pair_size, select64,
+from paged_util import (Paged, attend64, cu_of, forward_bound, half_step, norm_rotate64, pair_size, select64,
                         tables)
 
 pytestmark = pytest.mark.gpu
@@ -167,10 +167,10 @@ ATTENDS = [
 ]
 
 
-def check_attention(p, new, q, cfg, cache=None, tail=2, **more):
-    """Routing exact, outputs and lse within the bound, rows of no sequence untouched."""
-    g_cache, table, lens = p.gpu()
-    cache = cache or g_cache
+def check_attention(p, new, q, cfg, tail=2, tokens=None):
+    """Routing exact, outputs and lse within the bound, rows of no sequence untouched;
+    of all new tokens or those of a set."""
+    cache, table, lens = p.gpu()
     cu = cu_of(new).cuda()
     qg = torch.cat((q, torch.full((tail, *q.shape[1:]), math.nan, dtype=q.dtype))).cuda()
     ids = paged_gate_select(qg, cache, table, lens, cfg, cu_seqlens=cu).cpu()
@@ -181,6 +181,9 @@ def check_attention(p, new, q, cfg, cache=None, tail=2, **more):
     at = 0
     for s, n in enumerate(new):
         for i in range(n):
+            if tokens is not None and at not in tokens:
+                at += 1
+                continue
             pos = p.lens[s] - n + i
             want = select64(p, s, q[at], pos, cfg)
             for h, w in enumerate(want):
@@ -204,22 +207,130 @@ def test_attention(device, case):
     check_attention(p, new, q, cfg)
 
 
+# Chunks that go tile by tile and block by block: the same.
+CHUNKS = [
+    ([1000, 0, 333], [400, 100, 61], 8, 2, 128, BF, cfg_of(128, 4)),
+    ([1500], [300], 16, 4, 128, FH, cfg_of(64, 9)),
+    ([2000, 64, 7], [200, 64, 130], 16, 2, 64, FH, cfg_of(32, 17)),
+    ([300, 2500], [600, 40], 8, 8, 64, BF, cfg_of(96, 6)),
+    ([700, 70], [300, 250], 12, 4, 64, BF, cfg_of(128, 3, always_select_current=False)),
+    ([400, 200, 9], [500, 0, 77], 10, 2, 128, BF, cfg_of(100, 3, top_k_includes_current=False)),
+    ([900, 3], [300, 300], 8, 1, 256, BF, cfg_of(64, 3)),
+    ([1500], [400], 16, 4, 64, BF, cfg_of(16, 33)),
+    ([1100], [129], 128, 1, 128, FH, cfg_of(128, 2)),
+]
+
+
+def edges(p, new, n=24):
+    """First, last and some tokens of every chunk."""
+    out, at = set(), 0
+    for k in new:
+        out |= {at, at + k - 1} | {at + int(i) for i in torch.randint(0, k, (n,), generator=p.g)} if k else set()
+        at += k
+    return out
+
+
+def row_by_row(p, new, q, cfg):
+    """The chunk's tokens as many short calls, which take the single-token kernels."""
+    cache, table, _ = p.gpu()
+    ids, out, at = [], [], 0
+    for s, n in enumerate(new):
+        for i in range(0, n, 3):
+            m = min(3, n - i)
+            lens = torch.tensor([p.lens[s] - n + i + m], dtype=torch.int32, device="cuda")
+            part = q[at + i:at + i + m].cuda()
+            ids.append(paged_gate_select(part, cache, table[s:s + 1], lens, cfg))
+            out.append(paged_attention(part, cache, table[s:s + 1], lens, cfg))
+        at += n
+    return torch.cat(ids), torch.cat(out)
+
+
+def check_chunk(p, new, q, cfg, finite=True):
+    """Some tokens against 64 bits (where values are finite), all of them against
+    the single-token kernels."""
+    if finite:
+        check_attention(p, new, q, cfg, tokens=edges(p, new))
+    cache, table, lens = p.gpu()
+    cu = cu_of(new).cuda()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg, cu_seqlens=cu)
+    out = paged_attention(q.cuda(), cache, table, lens, cfg, cu_seqlens=cu)
+    given = paged_attention(q.cuda(), cache, table, lens, cfg, cu_seqlens=cu, block_idx=ids)
+    assert bool(((given == out) | (given.isnan() & out.isnan())).all())
+    want_ids, want = row_by_row(p, new, q, cfg)
+    assert torch.equal(ids, want_ids)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want.isposinf())
+    assert torch.equal(out.isneginf(), want.isneginf())
+    # Both round their result, block by block the weights too: half a step of
+    # the weighted mean of |v| each; codes and float32 sums are below 2^-14 of it.
+    most = p.v[p.v.isfinite()].abs().max().double()
+    far = torch.where(out.isfinite(), out.double() - want.double(), 0.0).abs().max()
+    assert far <= (3 * half_step(p.dtype) + 2.0 ** -13) * most
+
+
+@pytest.mark.parametrize("case", CHUNKS, ids=str)
+def test_chunks(device, case):
+    ctx, new, h, hk, d, dt, cfg = case
+    p = Paged([c + n for c, n in zip(ctx, new)], hk, cfg.block_size, d, dt, 13,
+              width=max(-(-(c + n) // cfg.block_size) for c, n in zip(ctx, new)) + 2)
+    check_chunk(p, new, p.randn(sum(new), h, d), cfg)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 6])
+def test_chunks_of_correlated_keys(device, dtype, size):
+    """Representatives that drift from block to block and lie far from zero:
+    neighbours score nearly alike, and many scores round to the same value."""
+    cfg = cfg_of(16, 12)
+    p = Paged([4000], 2, 16, 64, dtype, 14)
+    drift = torch.randn(p.kbar.shape[0], 2, 64, generator=p.g).cumsum(0) * 0.05 + 3
+    p.kbar[p.table[0, :250].long()] = (drift[:250] * size).to(dtype)
+    check_chunk(p, [300], p.randn(300, 16, 64) + 1, cfg)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+def test_chunks_without_pages(device, dtype):
+    cfg = cfg_of(128, 3)
+    new = [300, 1, 150]
+    p = Paged([1200, 1, 500], 2, 128, 128, dtype, 15)
+    p.table[0, 2], p.table[0, 5], p.table[0, 8] = -1, p.k.shape[0], 2 ** 31 - 1
+    p.table[1, 0] = -2
+    p.table[2, :4] = -1
+    check_chunk(p, new, p.randn(451, 12, 128), cfg)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("d,block", [(128, 128), (64, 96)])
+def test_chunks_with_special_values(device, dtype, d, block):
+    """Infinities and NaN, in values that all, some and none of the queries
+    see; a value of each where every query sees it; large values."""
+    cfg = cfg_of(block, 3)
+    n = 300
+    p = Paged([1000], 2, block, d, dtype, 16)
+    q = p.randn(n, 32, d)
+    p.v[p.v.isfinite()] *= 100
+    for row, feature, value in ((999, 3, math.nan), (998, 5, math.inf), (900, 7, -math.inf), (800, 9, math.nan),
+                                (650, d - 1, math.inf), (20, 0, -math.inf), (21, 0, math.inf), (5, 2, math.inf)):
+        p.v[p.table[0, row // block], :, row % block, feature] = value
+    check_chunk(p, [n], q, cfg, finite=False)
+
+
 @pytest.mark.parametrize("dtype", [BF, FH, F32])
-@pytest.mark.parametrize("new", [[1, 1], [40, 33]])
+@pytest.mark.parametrize("new", [[1, 1], [40, 33], [300, 290]])
 def test_ties_and_special_scores(device, dtype, new):
     """Integer-valued queries and keys (equal scores everywhere), and
     representatives with infinities and NaN."""
     cfg = cfg_of(16, 4)
     p = Paged([300 + new[0], 200 + new[1]], 2, 16, 64, dtype, 5)
-    q = torch.randint(-1, 2, (sum(new), 4, 64), generator=p.g).to(dtype)
+    q = torch.randint(-1, 2, (sum(new), 8, 64), generator=p.g).to(dtype)
+    tokens = edges(p, new) if sum(new) > 100 else None
     p.kbar[:] = torch.randint(-1, 2, p.kbar.shape, generator=p.g).to(dtype)
-    check_attention(p, new, q, cfg)
+    check_attention(p, new, q, cfg, tokens=tokens)
     p.kbar[p.table[0, 3], :, 5], p.kbar[p.table[0, 7], :, 5] = math.inf, -math.inf
     p.kbar[p.table[1, 2], :, 9], p.kbar[p.table[1, 4]] = math.nan, 0.0
-    check_attention(p, new, q, cfg)
+    check_attention(p, new, q, cfg, tokens=tokens)
     p.kbar[:] = torch.randn(p.kbar.shape, generator=p.g).to(dtype) * 2.0 ** -100 if dtype != FH else \
         torch.randn(p.kbar.shape, generator=p.g).to(dtype) * 2.0 ** -20
-    check_attention(p, new, q, cfg)
+    check_attention(p, new, q, cfg, tokens=tokens)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
