@@ -45,6 +45,12 @@ __device__ inline float row_lse(float top, float total) {
 // lane the best of every 64 NW-th score, every wave the best of its lanes, the
 // first wave the best of the waves (as select_kernel, without its launch and
 // its trip through memory).
+//
+// Memory-bound with many rows: one token of each of 32 sequences of up to 100k
+// keys, 32 and 8 heads of 128 in bf16, 8 blocks of 128 each: 96 us, 118 with the
+// scores, where the bytes of both take 94 at the rate of a large copy. One
+// sequence with 4 heads of 64 over 64k keys: 11 us, the latency of choosing
+// and of one pass.
 template <typename T, int D, int NW, int TM>
 __global__ void __launch_bounds__(64 * NW) attend_rows_kernel(RowArgs a) {
   constexpr int F = 16 / static_cast<int>(sizeof(T));

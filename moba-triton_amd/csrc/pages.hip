@@ -60,6 +60,11 @@ __device__ inline Piece find_piece(const Paged& p, int32_t piece) {
   return Piece{-1, 0, 0, 0};
 }
 
+// Memory-bound on prompts (5 of 1000 to 4096 tokens, 16 + 4 heads of 128 in
+// bf16: 33 us, 26 at the rate of a large copy); on single tokens of 64 sequences
+// 12 us, most of it the chain lengths -> table -> page -> keys of a block that
+// the token completes.
+//
 // One workgroup per run of new tokens on one page and (y) kv head, or four
 // query heads: y < h_kv writes K and V rows into the page and, where the run
 // fills the page's last row, the block's representative; the others write
@@ -216,7 +221,8 @@ struct CopyArgs {
 };
 
 // grid (pieces of a page's K, V and kbar, pairs, layers); a workgroup moves
-// kCopy pieces per thread, all in flight.
+// kCopy pieces per thread, all in flight. Memory-bound: 180 pages of 16 layers (8
+// heads, blocks of 128 x 128 in bf16, 3.0 GB) in 600 us, 5.1 TB/s; 8 pages in 27.
 constexpr int kCopy = 4;
 __global__ void __launch_bounds__(256) copy_kernel(CopyArgs a, CopyPairs list) {
   const int64_t pair = blockIdx.y;

@@ -7,5 +7,10 @@
     moba_bwd  the backward of the same
     attention the two halves as one differentiable operation
 
+and for generation:
+
+    rotary    norm and rotation of queries and keys, forward and backward
+    paged     the same over a paged cache: tokens appended, attended over, pages copied
+
 Every launcher calls the HIP library (`moba._lib`); none has a CPU path.
 """
