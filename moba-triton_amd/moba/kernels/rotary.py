@@ -184,6 +184,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
         k_weight = k_weight.contiguous()
     if positions is not None and (positions.dtype is not torch.int32 or positions.ndim != 2 or
                                   not positions.is_contiguous()):
+        if positions.dtype is torch.int64:  # far positions stay outside the tables
+            positions = positions.clamp(-1, 2 ** 31 - 1)
         positions = positions.to(torch.int32).expand(q.shape[:2]).contiguous()
     args = (q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), code)
     if torch.is_grad_enabled() and (

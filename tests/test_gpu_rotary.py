@@ -241,3 +241,12 @@ def test_zero_rows_without_eps_are_not_a_number(device):
     w = torch.ones(64, device="cuda")
     assert bool((norm_rotate(q, q, None, None, q_weight=w)[0] == 0).all())
     assert math.isnan(norm_rotate(q, q, None, None, q_weight=w, eps=0.0)[0].flatten()[0].item())
+
+
+def test_far_positions_are_outside_the_tables(device):
+    """int64 positions past 32 bits do not wrap around into the tables."""
+    q, k = torch.ones(1, 4, 1, 64, device="cuda"), torch.ones(1, 4, 1, 64, device="cuda")
+    cos, sin = (t.cuda() for t in tables(8, 64))
+    pos = torch.tensor([3, 2 ** 32 + 3, -2 ** 32 + 3, 2 ** 31], device="cuda")
+    for out in norm_rotate(q, k, cos, sin, positions=pos):
+        assert bool(out[0, 0].isfinite().all()) and bool(out[0, 1:].isnan().all())
