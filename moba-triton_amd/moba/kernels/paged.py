@@ -148,7 +148,10 @@ def append_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
             number for each. Tokens behind the last sequence are not read, and
             sequences whose numbers make no sense have no new tokens.
         cos, sin, q_weight, k_weight, eps, interleaved: As `norm_rotate`.
-        out: Receives the queries; rows of no sequence stay as they are.
+        out: Receives the queries; rows of no sequence stay as they are (and
+            hold anything without it).
+
+    No gradients (`norm_rotate` has them).
 
     Returns:
         The normed and rotated queries [T, H_q, D] (`out`).
@@ -256,7 +259,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor,
             shared. Blocks without a page hold no keys and are never selected.
         block_idx: The blocks of `paged_gate_select`, to attend to instead of
             the gate's choice: int32 [T, H_q, slots], no id twice in a row.
-        out: Receives the result; rows of no sequence stay as they are.
+        out: Receives the result; rows of no sequence stay as they are (and
+            hold anything without it, as their lse does).
+
+    No gradients: the cache's tokens are constants here.
 
     Returns:
         out [T, H_q, D], plus lse [H_q, T] float32 in log2 units when

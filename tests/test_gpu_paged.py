@@ -164,6 +164,8 @@ ATTENDS = [
     ([700, 2], [20, 40], 4, 2, 128, BF, cfg_of(32, 3, top_k_includes_current=False)),
     ([100] * 40 + [17], [1] * 40 + [130], 16, 2, 64, BF, cfg_of(32, 4)),
     ([50, 90] * 40, [1, 2] * 40, 2, 1, 64, BF, cfg_of(16, 3)),
+    ([3000, 1023], [1, 9], 4, 2, 64, BF, cfg_of(1024, 3)),
+    ([2100], [3], 2, 1, 256, F32, cfg_of(1024, 2)),
 ]
 
 
@@ -205,6 +207,14 @@ def test_attention(device, case):
               width=max(-(-(c + n) // cfg.block_size) for c, n in zip(ctx, new)) + 2)
     q = p.randn(sum(new), h, d)
     check_attention(p, new, q, cfg)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_wide_table(device, dtype):
+    """The widest table: its entries past the sequences' blocks do not count."""
+    cfg = cfg_of(16, 3)
+    p = Paged([270, 20], 2, 16, 64, dtype, 17, width=1 << 16)
+    check_attention(p, [70, 1], p.randn(71, 4, 64), cfg)
 
 
 # Chunks that go tile by tile and block by block: the same.
@@ -312,6 +322,74 @@ def test_chunks_with_special_values(device, dtype, d, block):
                                 (650, d - 1, math.inf), (20, 0, -math.inf), (21, 0, math.inf), (5, 2, math.inf)):
         p.v[p.table[0, row // block], :, row % block, feature] = value
     check_chunk(p, [n], q, cfg, finite=False)
+
+
+def test_replays_of_a_chunk(device):
+    """A captured chunk call replayed on other lengths, pages and queries, eager
+    calls and a second captured call between the replays."""
+    cfg = cfg_of(128, 4)
+    p = Paged([2000, 900], 2, 128, 128, BF, 18)
+    cache, table, lens = p.gpu()
+    q, cu = p.randn(400, 12, 128).cuda(), cu_of([250, 150]).cuda()
+    tables = [table, table.flip(1).contiguous(), table.roll(1, 1).contiguous(), table]
+    lengths = [lens, lens - 640, torch.tensor([260, 150], dtype=torch.int32, device="cuda"), lens]
+    cache.kbar.nan_to_num_(0.0)
+    cache.k.nan_to_num_(0.0)
+    cache.v.nan_to_num_(0.0)
+
+    def run(q, table, lens):
+        return paged_attention(q, cache, table, lens, cfg, cu_seqlens=cu, return_lse=True)
+
+    static = [t.clone() for t in (q, table, lens)]
+    run(*static)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(run(*static))
+            graphs.append(g)
+    torch.cuda.synchronize()
+    for i, (t, n) in enumerate(zip(tables, lengths)):
+        x = q.roll(i, 0)
+        want = run(x, t, n)
+        for buf, value in zip(static, (x, t, n)):
+            buf.copy_(value)
+        for g, (out, lse) in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), i
+            assert torch.equal(run(x, t, n)[0], want[0])
+
+
+def test_two_chunks_at_once(device):
+    cfg = cfg_of(128, 4)
+    p = Paged([1500], 2, 128, 128, FH, 19)
+    cache, table, lens = p.gpu()
+    qs = [p.randn(400, 12, 128).cuda() for _ in range(2)]
+    want = [paged_attention(q, cache, table, lens, cfg) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged_attention(qs[i], cache, table, lens, cfg))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_result_over_the_queries(device):
+    """`out` may be `q`: rows, split rows and chunks."""
+    for n, cfg in ((1, cfg_of(128, 9)), (400, cfg_of(128, 4))):
+        p = Paged([2500], 2, 128, 128, BF, 20)
+        cache, table, lens = p.gpu()
+        q = p.randn(n, 12, 128).cuda()
+        want = paged_attention(q, cache, table, lens, cfg)
+        assert torch.equal(paged_attention(q, cache, table, lens, cfg, out=q), want)
 
 
 @pytest.mark.parametrize("dtype", [BF, FH, F32])
