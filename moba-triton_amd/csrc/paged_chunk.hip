@@ -302,8 +302,13 @@ __device__ inline float of_special(int code) {
 // h, which the values' reads follow). P is rounded to the type for the
 // product, as the framework's forward does; m and l stay in float32. Partial
 // rows leave in halves of 64 features, as codes (Half).
+// kResident workgroups share a CU, as registers and LDS let them, and the grid
+// has as many: each has one item's loads under way.
+template <int D, int KT>
+constexpr int kResident = D * KT <= 64 ? 4 : D * KT <= 128 ? 3 : 2;
+
 template <typename T, int D, int KT>
-__global__ void __launch_bounds__(256, 2) attend_columns_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel(ChunkArgs a) {
   using M = Unit<T>;
   using V8 = typename M::vec;
   constexpr int KEYS = 32 * KT;
@@ -725,7 +730,8 @@ int chunk_attend(const moba_paged& c, const Paged& p, void* workspace, hipStream
     auto attend = [&](auto t, auto dim, auto kt) {
       using T = decltype(t);
       constexpr int D = decltype(dim)::value, KT = decltype(kt)::value;
-      const int64_t most = pl.max_items < 512 ? pl.max_items : 512;
+      constexpr int64_t kGrid = 256 * kResident<D, KT>;
+      const int64_t most = pl.max_items < kGrid ? pl.max_items : kGrid;
       hipLaunchKernelGGL((attend_columns_kernel<T, D, KT>), dim3(static_cast<unsigned>(most)), dim3(256), 0, s, a);
       int rc = check_launch("moba_paged_attend (attend)");
       if (rc) return rc;
