@@ -18,7 +18,7 @@
 // attention moves 0.67 GB, 3.8 TB/s: columns hold 64 entries on average, so half
 // of a workgroup's waves wait for the next block, and two workgroups share a CU's
 // LDS. 12 sequences with 1 to 700 tokens, 16 and 4 heads of 64 in fp16, 12 blocks
-// of 64: 23, 106 and 21 us.
+// of 64: 23, 97 and 21 us.
 //
 // An entry is its index in block_idx, which is also the index of its partial
 // row. Entries of a column stand in no particular order; nothing depends on it.
@@ -303,7 +303,8 @@ __device__ inline float of_special(int code) {
 // product, as the framework's forward does; m and l stay in float32. Partial
 // rows leave in halves of 64 features, as codes (Half).
 // kResident workgroups share a CU, as registers and LDS let them, and the grid
-// has as many: each has one item's loads under way.
+// has as many: each has one item's loads under way (D 64, blocks of 64, the fp16
+// call above: three 97 us, two 106; four would spill).
 template <int D, int KT>
 constexpr int kResident = D * KT <= 64 ? 4 : D * KT <= 128 ? 3 : 2;
 
