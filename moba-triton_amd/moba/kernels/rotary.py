@@ -153,7 +153,9 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                 eps: float = 1e-6, interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Queries and keys normed per head and rotated by position, with gradient
-    support for q, k and the weights. Computed in float32, rounded once.
+    support for q, k and the weights. Computed in float32, rounded once. In a
+    captured graph take the gradients with `torch.autograd.grad`, of leaves that
+    no live eager graph shares.
 
     Args:
         q: [B, S, H_q, D]; k: [B, S, H_kv, D]. Any strides (views of one fused
