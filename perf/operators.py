@@ -23,7 +23,6 @@ or by themselves; rotation of all features or of a part, of halves or of
 neighbours.
 """
 
-import functools
 import math
 import random
 import sys
@@ -37,10 +36,8 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 EPS = 1e-6
 
 
-@functools.cache
 def _package():
     # The package folder's name is no module name: its modules are found there.
-    # Once: a program imports before its first call, not with every call.
     pkg = str(Path.cwd() / "moba-triton_amd")
     if pkg not in sys.path:
         sys.path.insert(1, pkg)
