@@ -582,8 +582,9 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
     const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * a.h_q + hd) * a.slots;
     const float4* ml = a.part_ml + e0;
     const u32x4* acc = static_cast<const u32x4*>(a.part_acc) + e0 * LPR + c;
-    // Eight slots in flight. Those that were not written (m = -inf) hold
-    // anything: they count as zeros.
+    // Eight slots in flight. Those that were not written (m = -inf, l = 0) hold
+    // anything: they count as zeros. Where every score is NaN, m is -inf too (a
+    // maximum leaves NaN out) and l is NaN: the slot counts.
     float top = -INFINITY, total = 0.f, o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.f;
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
       float m = top;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (j0 + u >= a.slots) x[u].x = -INFINITY;
+        if (j0 + u >= a.slots) x[u] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
         m = fmaxf(m, x[u].x);
       }
       const float z = m > -INFINITY ? m : 0.f;
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
         constexpr bool kSpecial = decltype(with)::value;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const bool in = x[u].x != -INFINITY;
+          const bool in = x[u].x != -INFINITY || x[u].y != 0.f;
           const float w = __builtin_amdgcn_exp2f(x[u].x - z);
           total = fmaf(in ? x[u].y : 0.f, w, total);
           const float wu = in ? fabsf(c < 8 ? x[u].z : x[u].w) * w : 0.f;
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
       };
       bool special = false;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) special |= x[u].x != -INFINITY && fminf(x[u].z, x[u].w) < 0.f;
+      for (int u = 0; u < 8; ++u) special |= (x[u].x != -INFINITY || x[u].y != 0.f) && fminf(x[u].z, x[u].w) < 0.f;
       if (__any(special))
         add(std::true_type{});
       else

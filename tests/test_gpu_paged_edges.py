@@ -1,0 +1,70 @@
+"""Calls over a paged cache at the edges of what they take: scores that are not
+numbers."""
+
+import math
+
+import pytest
+import torch
+
+from moba.config import MoBAConfig
+from moba.kernels.paged import paged_attention, paged_gate_select
+from paged_util import Paged
+
+pytestmark = pytest.mark.gpu
+
+BF, FH, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def one_by_one(p, new, q, cfg):
+    """(ids, out, lse) of a chunk's tokens as short calls, which take the kernels
+    of single tokens."""
+    cache, table, _ = p.gpu()
+    ids, out, lse, at = [], [], [], 0
+    for s, n in enumerate(new):
+        for i in range(0, n, 3):
+            m = min(3, n - i)
+            lens = torch.tensor([p.lens[s] - n + i + m], dtype=torch.int32, device="cuda")
+            part = q[at + i:at + i + m].cuda()
+            ids.append(paged_gate_select(part, cache, table[s:s + 1], lens, cfg))
+            o, e = paged_attention(part, cache, table[s:s + 1], lens, cfg, return_lse=True)
+            out.append(o)
+            lse.append(e)
+        at += n
+    return torch.cat(ids), torch.cat(out), torch.cat(lse, 1)
+
+
+# -- scores that are not numbers --------------------------------------------------
+
+def check_scores_that_are_not_numbers(dtype, d, block, length, n, h, hk=2):
+    """Queries with NaN, a key of NaN that is the first of its token's own block,
+    a block whose keys are all NaN: whoever sees one has NaN for a result and for
+    its lse, and nobody else, as in short calls."""
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    p = Paged([length], hk, block, d, dtype, 21)
+    q = p.randn(n, h, d)
+    q[7, -1, 5], q[12], q[n - 1, 0] = math.nan, math.nan, math.nan
+    first = -(-(length - n) // block) * block  # a new token whose block begins with it
+    p.k[p.table[0, first // block], 0, 0, 9] = math.nan
+    p.k[p.table[0, 2], 1] = math.nan  # kbar stays: the block is chosen
+    cache, table, lens = p.gpu()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg)
+    out, lse = paged_attention(q.cuda(), cache, table, lens, cfg, return_lse=True)
+    want_ids, want, want_lse = one_by_one(p, [n], q, cfg)
+    assert torch.equal(ids, want_ids)
+    # By the definition: any NaN among the query and the keys that it sees.
+    pos = torch.arange(length - n, length)[:, None]
+    chosen, group = ids.cpu(), h // hk
+    bad = q.isnan().any(-1)
+    bad[:, :group] |= ((chosen == first // block).any(-1) & (pos >= first))[:, :group]
+    bad[:, group:] |= (chosen == 2).any(-1)[:, group:]
+    assert bool(bad[first - (length - n), :group].all()) and 0 < int(bad.sum()) < bad.numel()
+    for o, e in ((want, want_lse), (out, lse)):
+        assert torch.equal(o.cpu().isnan(), bad[..., None].expand(-1, -1, d))
+        assert torch.equal(e.cpu().isnan(), bad.t())
+        assert bool(o.cpu()[~bad].isfinite().all()) and bool(e.cpu().t()[~bad].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("d,block", [(128, 128), (64, 96)])
+def test_chunks_with_scores_that_are_not_numbers(device, dtype, d, block):
+    check_scores_that_are_not_numbers(dtype, d, block, 1000, 300, 32)
