@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
   const int32_t place0 = (lo - a.t0) * a.h_q * a.slots + hk * (hi - lo) * per;
   const uint32_t row = a.h_kv * a.p.width;  // the table has at most 2^22 entries, or one part per sequence
   int32_t* table = a.table + static_cast<int64_t>(first) * row + static_cast<int64_t>(hk) * a.p.width;
-  const int32_t blocks = min(a.p.width, (r.len + a.p.block - 1) / a.p.block);
+  const int32_t blocks = min(a.p.width, (r.len - 1) / a.p.block + 1);  // lengths up to 2^31 - 1
   // The columns' entries into LDS, and the number of items; then the lists.
   int32_t items = 0;
   for (int round = 0; round < 2; ++round) {

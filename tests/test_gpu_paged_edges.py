@@ -1,5 +1,5 @@
 """Calls over a paged cache at the edges of what they take: scores that are not
-numbers."""
+numbers, lengths and bounds that make no sense."""
 
 import math
 
@@ -8,7 +8,7 @@ import torch
 
 from moba.config import MoBAConfig
 from moba.kernels.paged import paged_attention, paged_gate_select
-from paged_util import Paged
+from paged_util import Paged, cu_of, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,31 @@ def check_scores_that_are_not_numbers(dtype, d, block, length, n, h, hk=2):
 @pytest.mark.parametrize("d,block", [(128, 128), (64, 96)])
 def test_chunks_with_scores_that_are_not_numbers(device, dtype, d, block):
     check_scores_that_are_not_numbers(dtype, d, block, 1000, 300, 32)
+
+
+# -- numbers that make no sense ---------------------------------------------------
+
+def check_farthest_length(dtype, d, block, ctx, new, h, hk=2):
+    """A sequence of 2^31 - 1 tokens between two ordinary ones: it sees its past
+    blocks, and they have every bit that they have beside an ordinary one."""
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    p = Paged([c + n for c, n in zip(ctx, new)], hk, block, d, dtype, 22,
+              width=max(-(-(c + n) // block) for c, n in zip(ctx, new)) + 2)
+    q = p.randn(sum(new), h, d)
+    cu = cu_of(new).cuda()
+    a, b = new[0], new[0] + new[1]
+    cache, table, lens = p.gpu()
+    want = paged_attention(q.cuda(), cache, table, lens, cfg, cu_seqlens=cu)
+    p.lens[1] = 2 ** 31 - 1
+    cache, table, lens = p.gpu()
+    out = paged_attention(q.cuda(), cache, table, lens, cfg, cu_seqlens=cu)
+    assert torch.equal(out[:a], want[:a]) and torch.equal(out[b:], want[b:])
+    alone = one_by_one(p, new, q, cfg)[1]
+    # Weights and results rounded, half a step of max |v| each on each side.
+    far = (out[a:b].double() - alone[a:b].double()).abs().max().item()
+    assert far <= 4 * half_step(dtype) * p.v[p.v.isfinite()].abs().max().item()
+
+
+@pytest.mark.parametrize("dtype,d,block", [(BF, 128, 128), (FH, 64, 64)])
+def test_the_farthest_length_in_a_chunk(device, dtype, d, block):
+    check_farthest_length(dtype, d, block, [900, 300, 700], [200, 60, 150], 32)
