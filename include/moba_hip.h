@@ -361,9 +361,11 @@ int moba_norm_rotate_bwd(const void* dq_out, const void* dk_out, const void* q, 
  * sequence's tokens with its new ones, which are its last. cu_seqlens [seqs +
  * 1] int32 packs the new tokens along the token axis (a sequence may have
  * none); NULL: `even` tokens each. Rows of the token axis that belong to no
- * sequence are neither read nor written, and sequences whose numbers make no
+ * sequence are neither read nor written. A sequence whose numbers make no
  * sense (cu_seqlens outside the token axis or falling, seq_lens below the new
- * tokens) have no new tokens. All of this is read on the device.
+ * tokens), or whose tokens begin before an earlier one's end whose numbers do,
+ * has no new tokens; the others are served as without it. All of this is read
+ * on the device.
  * Pages of one call's sequences that are appended to must be distinct; pages
  * that are only read may be shared.
  * head_dim 64, 128 or 256; block_size up to 1024; everything on 16-byte

@@ -40,6 +40,28 @@ __device__ inline NewTokens new_tokens(const Paged& p, int32_t s) {
   return checked_tokens(p, first, p.cu ? p.cu[s + 1] : first + p.even, p.seq_lens[s]);
 }
 
+// The same for the sequences base, base + 1, .. of a wave's lanes (n 0 past the
+// last), one call after another from base 0 on: a sequence counts only where no
+// earlier one that makes sense by itself reaches behind its first token, so
+// that no token has two sequences and their tokens are at most p.tokens in all.
+// `reach`: where the earlier ones end, 0 at first.
+__device__ inline NewTokens counted_tokens(const Paged& p, int32_t base, int32_t& reach) {
+  const int lane = threadIdx.x & 63;
+  NewTokens r{0, 0, 0};
+  if (base + lane < p.seqs) r = new_tokens(p, base + lane);
+  if (!p.cu) return r;
+  int32_t end = r.n ? r.first + r.n : 0;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int32_t y = __shfl_up(end, off);
+    if (lane >= off) end = max(end, y);
+  }
+  const int32_t up = __shfl_up(end, 1), before = max(reach, lane ? up : 0);
+  if (r.first < before) r.n = 0;
+  reach = max(reach, __shfl(end, 63));
+  return r;
+}
+
 // Sequence and position of token `tok`, the same in all lanes of the wave;
 // position -1 where the token belongs to no sequence (rows behind the last
 // one, inconsistent lengths). Every lane holds the numbers of one of 64
@@ -59,14 +81,26 @@ __device__ inline TokenAt locate(const Paged& p, int32_t tok) {
     return token_at(s, new_tokens(p, s), tok);
   }
   const int lane = threadIdx.x & 63;
+  int32_t reach = 0;
   for (int32_t base = 0; base < p.seqs; base += 64) {
-    const int32_t i = min(base + lane, p.seqs - 1);
-    const int32_t first = p.cu[i], end = p.cu[i + 1], len = p.seq_lens[i];
-    // Sequences up to the one that holds the token end at or before it.
-    const uint64_t behind = __ballot(base + lane < p.seqs && end > tok);
-    if (!behind) continue;
-    const int l = __builtin_ctzll(behind);
-    return token_at(base + l, checked_tokens(p, __shfl(first, l), __shfl(end, l), __shfl(len, l)), tok);
+    NewTokens r = new_tokens(p, min(base + lane, p.seqs - 1));
+    if (base + lane >= p.seqs) r.n = 0;
+    const int32_t end = r.n ? r.first + r.n : 0;
+    const uint64_t holds = __ballot(r.first <= tok && tok < end);
+    if (holds) {
+      // As counted_tokens: the first one that holds the token or none, for it
+      // reaches behind the first tokens of the others that do.
+      const int l = __builtin_ctzll(holds);
+      const int32_t first = __shfl(r.first, l);
+      if (first < reach || __ballot(lane < l && end > first)) break;
+      return token_at(base + l, NewTokens{first, __shfl(r.n, l), __shfl(r.len, l)}, tok);
+    }
+    if (base + 64 < p.seqs) {
+      int32_t most = end;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off));
+      reach = max(reach, most);
+    }
   }
   return TokenAt{0, -1};
 }

@@ -116,28 +116,26 @@ __global__ void __launch_bounds__(1024) column_scan_kernel(ChunkArgs a) {
   const int hk = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // This sequence's parts and where its entries begin.
-  const NewTokens r = new_tokens(a.p, seq);
-  const int32_t lo = max(r.first, a.t0), hi = min(r.first + r.n, a.t1);
-  if (hi <= lo) return;
-  int32_t first = 0;
-  for (int32_t base = 0; base < seq; base += 64) {
-    int32_t mine = 0;
-    if (base + lane < seq) {
-      const NewTokens o = new_tokens(a.p, base + lane);
-      const int32_t l = max(o.first, a.t0), h = min(o.first + o.n, a.t1);
-      mine = h > l ? (h - l + a.part - 1) / a.part : 0;
-    }
+  int32_t first = 0, lo = 0, hi = 0, len = 0, reach = 0;
+  for (int32_t base = 0; base <= seq; base += 64) {
+    const NewTokens o = counted_tokens(a.p, base, reach);
+    const int32_t l = max(o.first, a.t0), h = min(o.first + o.n, a.t1);
+    int32_t mine = base + lane < seq && h > l ? (h - l + a.part - 1) / a.part : 0;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) mine += __shfl_xor(mine, off);
     first += mine;
+    const int at = seq - base;  // below 64 in the last round
+    lo = __shfl(l, at & 63);
+    hi = __shfl(h, at & 63);
+    len = __shfl(o.len, at & 63);
   }
+  if (hi <= lo) return;
   const int32_t parts = (hi - lo + a.part - 1) / a.part;
-  if (first + parts > a.parts) return;  // only where sequences claim the same tokens
   const int per = a.h_q / a.h_kv * a.slots;
   const int32_t place0 = (lo - a.t0) * a.h_q * a.slots + hk * (hi - lo) * per;
   const uint32_t row = a.h_kv * a.p.width;  // the table has at most 2^22 entries, or one part per sequence
   int32_t* table = a.table + static_cast<int64_t>(first) * row + static_cast<int64_t>(hk) * a.p.width;
-  const int32_t blocks = min(a.p.width, (r.len - 1) / a.p.block + 1);  // lengths up to 2^31 - 1
+  const int32_t blocks = min(a.p.width, (len - 1) / a.p.block + 1);  // lengths up to 2^31 - 1
   // The columns' entries into LDS, and the number of items; then the lists.
   int32_t items = 0;
   for (int round = 0; round < 2; ++round) {

@@ -148,10 +148,9 @@ struct Part {
 
 __device__ inline Part find_part(const Paged& p, int32_t t0, int32_t t1, int32_t size, int32_t part) {
   const int lane = threadIdx.x & 63;
-  int32_t before = 0;
+  int32_t before = 0, reach = 0;
   for (int32_t base = 0; base < p.seqs; base += 64) {
-    NewTokens r{0, 0, 0};
-    if (base + lane < p.seqs) r = new_tokens(p, base + lane);
+    const NewTokens r = counted_tokens(p, base, reach);
     const int32_t lo = max(r.first, t0), hi = min(r.first + r.n, t1);
     const int32_t mine = hi > lo ? (hi - lo + size - 1) / size : 0;
     int32_t upto = mine;

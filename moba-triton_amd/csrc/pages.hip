@@ -29,11 +29,9 @@ struct Piece {
 
 __device__ inline Piece find_piece(const Paged& p, int32_t piece) {
   const int lane = threadIdx.x & 63;
-  int32_t before = 0;
+  int32_t before = 0, reach = 0;
   for (int32_t base = 0; base < p.seqs; base += 64) {
-    const int32_t s = base + lane;
-    NewTokens r{0, 0, 0};
-    if (s < p.seqs) r = new_tokens(p, s);
+    const NewTokens r = counted_tokens(p, base, reach);
     const int32_t lo = r.len - r.n;
     const int32_t mine = r.n ? (r.len - 1) / p.block - lo / p.block + 1 : 0;
     int32_t upto = mine;  // inclusive sum over the lanes

@@ -145,8 +145,10 @@ def append_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
         seq_lens: int32 [sequences], tokens of each sequence with its new ones.
         cu_seqlens: int32 [sequences + 1], where each sequence's new tokens
             begin on the token axis (a sequence may have none); None: the same
-            number for each. Tokens behind the last sequence are not read, and
-            sequences whose numbers make no sense have no new tokens.
+            number for each. Tokens behind the last sequence are not read.
+            A sequence whose numbers make no sense (outside the token axis,
+            falling, more new tokens than `seq_lens`), or that begins before
+            an earlier one's end, has no new tokens; the others are served.
         cos, sin, q_weight, k_weight, eps, interleaved: As `norm_rotate`.
         out: Receives the queries; rows of no sequence stay as they are (and
             hold anything without it).

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from moba.config import MoBAConfig
-from moba.kernels.paged import paged_attention, paged_gate_select
+from moba.kernels.paged import append_tokens, paged_attention, paged_gate_select
 from paged_util import Paged, cu_of, half_step
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +96,61 @@ def check_farthest_length(dtype, d, block, ctx, new, h, hk=2):
 @pytest.mark.parametrize("dtype,d,block", [(BF, 128, 128), (FH, 64, 64)])
 def test_the_farthest_length_in_a_chunk(device, dtype, d, block):
     check_farthest_length(dtype, d, block, [900, 300, 700], [200, 60, 150], 32)
+
+
+def check_bounds(dtype, d, block, bounds, counted, tokens, ctx, h, hk=2):
+    """Bounds that fall, leave the token axis or overlap: sequences that make
+    sense by themselves and begin where no earlier such one reaches are served,
+    the others have no new tokens, in every call alike."""
+    seqs = len(bounds) - 1
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    new = [max(0, b - a) if b <= tokens else 7 for a, b in zip(bounds, bounds[1:])]
+    p = Paged([ctx + n for n in new], hk, block, d, dtype, 23, width=-(-(ctx + max(new)) // block) + 1)
+    x = p.randn(tokens, h + 2 * hk, d).cuda()
+    q, k, v = x[:, :h], x[:, h:h + hk], x[:, h + hk:]
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    cache, table, lens = p.gpu()
+    want_cache, _, _ = p.gpu()
+    mine = torch.zeros(tokens, dtype=torch.bool)
+    for s in counted:
+        mine[bounds[s]:bounds[s + 1]] = True
+    mine = mine.to(q.device)
+    out = torch.full((tokens, h, d), 5.0, dtype=dtype, device="cuda")
+    append_tokens(q, k, v, cache, table, lens, cu_seqlens=cu, out=out)
+    assert torch.equal(out[mine], q[mine]) and bool((out[~mine] == 5).all())
+    ids = paged_gate_select(q, cache, table, lens, cfg, cu_seqlens=cu)
+    out.fill_(5.0)
+    _, lse = paged_attention(q, cache, table, lens, cfg, cu_seqlens=cu, out=out, return_lse=True)
+    assert bool((out[~mine] == 5).all()) and bool((ids[~mine] == -1).all())
+    for s in counted:
+        at = slice(bounds[s], bounds[s + 1])
+        one = (table[s:s + 1].contiguous(), lens[s:s + 1])
+        append_tokens(q[at], k[at], v[at], want_cache, *one)
+        assert torch.equal(ids[at], paged_gate_select(q[at], want_cache, *one, cfg))
+        want, want_lse = paged_attention(q[at], want_cache, *one, cfg, return_lse=True)
+        # Weights and results rounded, half a step of max |v| each on each
+        # side; float32: sums of up to 4 blocks in any order.
+        most = p.v[p.v.isfinite()].abs().max().item()
+        bar = 4 * half_step(dtype) * most if dtype != F32 else 2.0 ** -24 * 8 * block * most
+        assert (out[at].double() - want.double()).abs().max().item() <= bar
+        assert (lse[:, at] - want_lse).abs().max().item() <= 1e-4 + 2.0 ** -7 * (dtype != F32)
+    for name in ("k", "v", "kbar"):
+        a, b = (getattr(c, name).view(torch.uint8) for c in (cache, want_cache))
+        assert torch.equal(a, b), name
+
+
+# bounds, sequences that count
+BOUNDS = [
+    ([0, 999, 20, 60, 60], [2]),                       # the first leaves the axis
+    ([0, 50, 30, 70, 100], [0, 3]),                    # the third begins inside the first
+    ([-3, 10, 90, 5, 100], [1]),                       # the last begins before the second ends
+    ([0, 40, 10, 100, 70, 90], [0]),                   # and so do all behind the first
+    ([0] * 66 + [30, 20, 60, 100], [65, 68]),          # across 64 sequences
+]
+
+
+@pytest.mark.parametrize("bounds,counted", BOUNDS, ids=str)
+@pytest.mark.parametrize("dtype,d,block", [(BF, 128, 128), (FH, 64, 64), (F32, 64, 32)])
+@pytest.mark.parametrize("scale,h", [(1, 4), (3, 32)])
+def test_bounds_that_make_no_sense(device, dtype, d, block, bounds, counted, scale, h):
+    check_bounds(dtype, d, block, [scale * b for b in bounds], counted, 100 * scale, 700, h)
