@@ -17,8 +17,8 @@ struct ChunkArgs {
   int32_t* table;            // [parts, h_kv, width]
   int4* items;               // (sequence * h_kv + kv head, block, first entry's place, entries)
   int32_t* entries;          // indices into the slice's [tokens, h_q, slots]
-  float4* part_ml;           // (m, l, units of the row's halves) per entry
-  void* part_acc;            // [entries, D] in codes of 16 bits
+  float2* part_ml;           // (m, l) per entry
+  float* part_acc;           // [entries, D]
   int32_t t0, t1;            // tokens of this slice
   int h_q, h_kv, slots;
   int part, parts, max_items;

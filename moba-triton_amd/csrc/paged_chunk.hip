@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kSortThreads) column_place_kernel(ChunkArgs a)
       if (blk[u] >= 0)
         a.entries[atomicAdd(&cursor[blk[u]], 1)] = e[u];
       else if (i0 + kSortThreads * u < n)
-        a.part_ml[e[u]] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        a.part_ml[e[u]] = make_float2(-INFINITY, 0.f);
     }
   }
 }
@@ -235,71 +235,16 @@ __device__ inline int swizzle_v(int row) {
   return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row >> 1) & 1) << 2;
 }
 
-// A half of a partial row, 64 features, as whole numbers of 16 bits and a unit
-// that is 1/32700 of the half's largest magnitude: half the bytes of float32 at
-// an error below 2^-16 of that largest, where rounding to bf16 is off by up to
-// 2^-9 of every element (a query's 8 partial rows then added as much error as
-// the rounding of the result does, at no less traffic).
-// A half with infinities or NaN has a negative unit and codes for them.
-constexpr int kCodes = 32700, kInfCode = 32767, kNanCode = 0x8000;
-constexpr float kLeast = 0x1p-110f;  // largest magnitudes below it count as it
-
-__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one is
-
-__device__ inline uint32_t special_code(float x, uint32_t code) {
-  if (x != x) return kNanCode;
-  return fabsf(x) < INFINITY ? code : (x > 0.f ? kInfCode : -kInfCode) & 0xffffu;
-}
-
-// o[t][i], 32 features of the lane; lane ^ 32 has the others.
-__device__ inline float half_codes(const floatx16_t (&o)[2], u32x2 (&code)[2][4]) {
-  float top = 0.f;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = larger(top, fabsf(o[t][i]));
-  top = larger(top, __shfl_xor(top, 32));
-  const bool strange = !(top < INFINITY);
-  const bool any = __any(strange);
-  if (any) {
-    float finite = 0.f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) finite = fmaxf(finite, fabsf(o[t][i]) < INFINITY ? fabsf(o[t][i]) : 0.f);
-    top = fmaxf(finite, __shfl_xor(finite, 32));
-  }
-  top = fmaxf(top, kLeast);
-  // The conversion multiplies by 32767 and rounds to the nearest.
-  const float per = (kCodes / 32767.f) * __builtin_amdgcn_rcpf(top);
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const float x = o[t][4 * q4 + 2 * w], y = o[t][4 * q4 + 2 * w + 1];
-        uint32_t c = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(x * per, y * per));
-        if (any) c = special_code(x, c & 0xffffu) | (special_code(y, c >> 16) << 16);
-        code[t][q4][w] = c;
-      }
-  const float unit = top * (1.f / kCodes);
-  return strange ? -unit : unit;
-}
-
-__device__ inline float of_special(int code) {
-  if (code > -kInfCode && code < kInfCode) return static_cast<float>(code);
-  return code < -kInfCode ? NAN : code > 0 ? INFINITY : -INFINITY;
-}
-
 // KT tiles of 32 keys cover the block. A wave holds 32 entries, one per lane
 // pair (lane, lane ^ 32):
 //   S^T[key][entry] = K . Q^T,   O^T[feature][entry] = V^T . P^T
 // by 32x32x16 MFMAs; P^T goes from the first product's registers to the
 // second's operand (its keys in the order 8 (u / 4) + 4 h + u % 4 of lane half
 // h, which the values' reads follow). P is rounded to the type for the
-// product, as the framework's forward does; m and l stay in float32. Partial
-// rows leave in halves of 64 features, as codes (Half).
+// product, as the framework's forward does; m, l and the partial rows stay in
+// float32. (Rows as 16-bit codes with a unit per 64 features move half the bytes
+// and coarsen the features beside a large one: values with one channel of 64
+// 1000 times the others' came out 0.9% off.)
 // kResident workgroups share a CU, as registers and LDS let them, and the grid
 // has as many: each has one item's loads under way (D 64, blocks of 64, the fp16
 // call above: three 97 us, two 106; four would spill).
@@ -512,20 +457,19 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
         meet();
       }
     }
-    // Two feature tiles at a time, encoded and kept until the queries are in.
-    u32x2 rows[DT / 2][2][4];
-    float units[2] = {0.f, 0.f};
+    // Two feature tiles at a time, kept until the queries are in.
+    floatx16_t o[DT];
     if (work) {
       auto half = [&](auto pc) {
-        constexpr int half_row = decltype(pc)::value, dt = 2 * half_row;
-        floatx16_t o[2] = {floatx16_t{}, floatx16_t{}};
+        constexpr int dt = 2 * decltype(pc)::value;
+        o[dt] = o[dt + 1] = floatx16_t{};
         // Features 32 dt + [0, 64), keys 16 j + [0, 16).
         auto step = [&](auto jc) {
           constexpr int j = decltype(jc)::value;
           u32x2 x[4];
           read_transposed<64 * dt, j * 16 * D * 2>(v_at, v_at8, x);
-          o[0] = M::mma(__builtin_bit_cast(V8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]}), bp[j], o[0]);
-          o[1] = M::mma(__builtin_bit_cast(V8, u32x4{x[2][0], x[2][1], x[3][0], x[3][1]}), bp[j], o[1]);
+          o[dt] = M::mma(__builtin_bit_cast(V8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]}), bp[j], o[dt]);
+          o[dt + 1] = M::mma(__builtin_bit_cast(V8, u32x4{x[2][0], x[2][1], x[3][0], x[3][1]}), bp[j], o[dt + 1]);
         };
         steps(std::make_integer_sequence<int, KEYS / 16>{}, step);
         if (bad) {
@@ -541,24 +485,24 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
                 for (int w = 0; w < 4; ++w) {
                   const uint16_t bits = static_cast<uint16_t>(x[w >> 1] >> (16 * (w & 1)));
                   if ((bits & M::kInf) == M::kInf && key <= lim)
-                    o[t][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
+                    o[dt + t][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
                 }
               }
           }
         }
-        units[half_row] = half_codes(o, rows[half_row]);
       };
       steps(std::make_integer_sequence<int, DT / 2>{}, half);
     }
     have_query();
     if (live && work) {
-      if (h == 0) a.part_ml[ent] = make_float4(m, l, units[0], units[1]);
-      uint16_t* dst = static_cast<uint16_t*>(a.part_acc) + static_cast<int64_t>(ent) * D + 4 * h;
+      if (h == 0) a.part_ml[ent] = make_float2(m, l);
+      float* dst = a.part_acc + static_cast<int64_t>(ent) * D + 4 * h;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<u32x2*>(dst + dt * 32 + 8 * q4) = rows[dt / 2][dt % 2][q4];
+          *reinterpret_cast<float4*>(dst + dt * 32 + 8 * q4) =
+              make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
     }
     meet();  // every wave is done with the values
     if (!more) break;
@@ -578,8 +522,8 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
   const int c = threadIdx.x % LPR;
   for (int hd = threadIdx.x / LPR; hd < a.h_q; hd += blockDim.x / LPR) {
     const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * a.h_q + hd) * a.slots;
-    const float4* ml = a.part_ml + e0;
-    const u32x4* acc = static_cast<const u32x4*>(a.part_acc) + e0 * LPR + c;
+    const float2* ml = a.part_ml + e0;
+    const float4* acc = reinterpret_cast<const float4*>(a.part_acc + e0 * D) + 2 * c;
     // Eight slots in flight. Those that were not written (m = -inf, l = 0) hold
     // anything: they count as zeros. Where every score is NaN, m is -inf too (a
     // maximum leaves NaN out) and l is NaN: the slot counts.
@@ -587,18 +531,19 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.f;
     for (int j0 = 0; j0 < a.slots; j0 += 8) {
-      float4 x[8];
-      u32x4 raw[8];
+      float2 x[8];
+      float4 raw[8][2];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int j = min(j0 + u, a.slots - 1);
         x[u] = ml[j];
-        raw[u] = acc[j * LPR];
+        raw[u][0] = acc[j * (D / 4)];
+        raw[u][1] = acc[j * (D / 4) + 1];
       }
       float m = top;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (j0 + u >= a.slots) x[u] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        if (j0 + u >= a.slots) x[u] = make_float2(-INFINITY, 0.f);
         m = fmaxf(m, x[u].x);
       }
       const float z = m > -INFINITY ? m : 0.f;
@@ -606,29 +551,16 @@ __global__ void __launch_bounds__(512) merge_slots_kernel(ChunkArgs a) {
       total *= old;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] *= old;
-      auto add = [&](auto with) {
-        constexpr bool kSpecial = decltype(with)::value;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const bool in = x[u].x != -INFINITY || x[u].y != 0.f;
-          const float w = __builtin_amdgcn_exp2f(x[u].x - z);
-          total = fmaf(in ? x[u].y : 0.f, w, total);
-          const float wu = in ? fabsf(c < 8 ? x[u].z : x[u].w) * w : 0.f;
-          const bool mine = kSpecial && in && (c < 8 ? x[u].z : x[u].w) < 0.f;
+      for (int u = 0; u < 8; ++u) {
+        const bool in = x[u].x != -INFINITY || x[u].y != 0.f;
+        const float w = __builtin_amdgcn_exp2f(x[u].x - z);
+        total = fmaf(x[u].y, w, total);
+        const float v[8] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w,
+                            raw[u][1].x, raw[u][1].y, raw[u][1].z, raw[u][1].w};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int code = static_cast<int16_t>(raw[u][e >> 1] >> (16 * (e & 1)));
-            o[e] = fmaf(mine ? of_special(code) : static_cast<float>(code), wu, o[e]);
-          }
-        }
-      };
-      bool special = false;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) special |= (x[u].x != -INFINITY || x[u].y != 0.f) && fminf(x[u].z, x[u].w) < 0.f;
-      if (__any(special))
-        add(std::true_type{});
-      else
-        add(std::false_type{});
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(in ? v[e] : 0.f, w, o[e]);
+      }
       top = m;
     }
     const int64_t row = static_cast<int64_t>(tok) * a.h_q + hd;
@@ -667,7 +599,7 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   ChunkPlan pl;
   const int64_t per_token = c.h_q * c.slots;
   // Partial rows of at most 2^29 bytes at a time.
-  pl.slice = (int64_t(1) << 29) / (per_token * c.head_dim * 2);
+  pl.slice = (int64_t(1) << 29) / (per_token * c.head_dim * 4);
   pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
   // Parts of 64 tokens: more workgroups count and place, and the scan walks more
   // parts (4 x 512 tokens, 4 kv heads: the attention 157 us, in parts of 256
@@ -686,8 +618,8 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   pl.table = take(sizeof(int32_t) * static_cast<size_t>(pl.parts * row));
   pl.items = take(sizeof(int4) * static_cast<size_t>(pl.max_items));
   pl.entries = take(sizeof(int32_t) * static_cast<size_t>(entries));
-  pl.ml = take(sizeof(float4) * static_cast<size_t>(entries));
-  pl.acc = take(sizeof(int16_t) * static_cast<size_t>(entries * c.head_dim));
+  pl.ml = take(sizeof(float2) * static_cast<size_t>(entries));
+  pl.acc = take(sizeof(float) * static_cast<size_t>(entries * c.head_dim));
   pl.total = o;
   return pl;
 }
@@ -707,8 +639,8 @@ int chunk_attend(const moba_paged& c, const Paged& p, void* workspace, hipStream
   a.table = reinterpret_cast<int32_t*>(ws + pl.table);
   a.items = reinterpret_cast<int4*>(ws + pl.items);
   a.entries = reinterpret_cast<int32_t*>(ws + pl.entries);
-  a.part_ml = reinterpret_cast<float4*>(ws + pl.ml);
-  a.part_acc = ws + pl.acc;
+  a.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
+  a.part_acc = reinterpret_cast<float*>(ws + pl.acc);
   a.h_q = static_cast<int>(c.h_q);
   a.h_kv = static_cast<int>(c.h_kv);
   a.slots = static_cast<int>(c.slots);

@@ -154,3 +154,76 @@ BOUNDS = [
 @pytest.mark.parametrize("scale,h", [(1, 4), (3, 32)])
 def test_bounds_that_make_no_sense(device, dtype, d, block, bounds, counted, scale, h):
     check_bounds(dtype, d, block, [scale * b for b in bounds], counted, 100 * scale, 700, h)
+
+
+# -- values of very different sizes -----------------------------------------------
+
+def attend_exactly(p, q, ids, pos):
+    """One query's head of a kv head 0 .. by 64 bits: (out, weighted mean of |v|,
+    largest |v| of each feature, bound on a weight's relative error by float32).
+
+    Scores: at most D / 8 + 8 additions of one chain and two products, of sums
+    of |q k| scaled; twice, in the row and in its sum; exp2 and the sums over
+    keys and blocks, 64 roundings more."""
+    ks, vs = [], []
+    for j in ids:
+        page, seen = int(p.table[0, j]), min(p.block, pos - j * p.block + 1)
+        ks.append(p.k[page, :, :seen].double())
+        vs.append(p.v[page, :, :seen].double())
+    k, v = torch.cat(ks, 1), torch.cat(vs, 1)
+    scale = q.shape[-1] ** -0.5
+    w = torch.softmax((k[0] @ q.double()) * scale, 0)
+    terms = (k[0].abs() @ q.double().abs()).max().item() * scale
+    delta = 2 * 2.0 ** -24 * ((q.shape[-1] / 8 + 24) * terms + 64)
+    return w @ v[0], w @ v[0].abs(), v[0].abs().amax(0), delta
+
+
+def check_values(p, q, cfg, weights, tokens):
+    """Every feature of a chunk's result (one kv head) within its own bound: half
+    a step of the result, `weights` of the weighted mean of |v|, float32 sums."""
+    n, h, d = q.shape
+    cache, table, lens = p.gpu()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg).cpu()
+    out = paged_attention(q.cuda(), cache, table, lens, cfg).cpu().double()
+    for i in tokens:
+        for hd in range(h):
+            pos = p.lens[0] - n + i
+            ref, mean, most, delta = attend_exactly(p, q[i, hd], [j for j in ids[i, hd].tolist() if j >= 0], pos)
+            bound = half_step(p.dtype) * ref.abs() + weights * mean + delta * most
+            if p.dtype == FH:
+                bound = bound + 2.0 ** -25
+            far = (out[i, hd] - ref).abs()
+            assert bool((far <= bound).all()), (i, hd, (far / bound).max().item())
+
+
+def check_large_channels(dtype, d, block, length, n, h, ratio):
+    """A feature of every 64 that is `ratio` times the others leaves them as
+    exact as they are without it."""
+    p = Paged([length], 1, block, d, dtype, 24)
+    p.v[..., 5] *= ratio
+    p.v[..., d - 9] *= ratio
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    check_values(p, p.randn(n, h, d), cfg, half_step(dtype), range(0, n, max(1, n // 12)))
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("d,block", [(128, 128), (64, 96)])
+@pytest.mark.parametrize("ratio", [100, 4000])
+def test_large_channels_leave_the_others_exact(device, dtype, d, block, ratio):
+    check_large_channels(dtype, d, block, 1000, 300, 16, ratio)
+
+
+def check_largest_values(block, length, n, h):
+    """bf16 values behind 2^126, whose reciprocals are subnormal: one key of
+    every block, at most three blocks to a query, so no sum passes float32."""
+    p = Paged([length], 1, block, 64, BF, 25)
+    p.v[p.v.isfinite()] = 0.0
+    for j in range(length // block):
+        p.v[p.table[0, j], 0, j % 3, 3] = 1e38
+        p.v[p.table[0, j], 0, j % 5, 40] = -9e37
+    cfg = MoBAConfig(block_size=block, top_k=3)
+    check_values(p, p.randn(n, h, 64), cfg, half_step(BF), range(0, n, max(1, n // 12)))
+
+
+def test_the_largest_values_in_a_chunk(device):
+    check_largest_values(64, 1500, 600, 32)
