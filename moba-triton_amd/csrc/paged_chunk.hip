@@ -408,13 +408,15 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) m = fmaxf(m, s[kt][v]);
-      m = fmaxf(m, __shfl_xor(m, 32)) * a.scale_log2;
+      m = fmaxf(m, __shfl_xor(m, 32));
       const float mz = m > -INFINITY ? m : 0.f;
+      m *= a.scale_log2;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[kt][v], a.scale_log2, -mz));
+          // The difference first: at most 1 however large the scores are.
+          const float p = __builtin_amdgcn_exp2f((s[kt][v] - mz) * a.scale_log2);
           s[kt][v] = p;
           l += p;
         }

@@ -227,3 +227,43 @@ def check_largest_values(block, length, n, h):
 
 def test_the_largest_values_in_a_chunk(device):
     check_largest_values(64, 1500, 600, 32)
+
+
+def check_far_scores(dtype, block, length, n, h, size):
+    """Scores so large that neighbours are far apart in float32: nothing but the
+    best key of every query counts, and no weight leaves the type's range."""
+    d = 64
+    p = Paged([length], 1, block, d, dtype, 27)
+    real = p.k.isfinite()
+    p.k[real] = (p.k[real].float() * size).to(dtype)
+    q = (p.randn(n, h, d).float() * size).to(dtype)
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    cache, table, lens = p.gpu()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg).cpu()
+    out, lse = paged_attention(q.cuda(), cache, table, lens, cfg, return_lse=True)
+    assert bool(out.isfinite().all()) and bool(lse.isfinite().all())
+    out = out.cpu().double()
+    sure = 0
+    for i in range(0, n, max(1, n // 25)):
+        for hd in range(h):
+            ks, vs = [], []
+            for j in (j for j in ids[i, hd].tolist() if j >= 0):
+                page, seen = int(p.table[0, j]), min(block, length - n + i - j * block + 1)
+                ks.append(p.k[page, 0, :seen].double())
+                vs.append(p.v[page, 0, :seen].double())
+            k, v = torch.cat(ks), torch.cat(vs)
+            x = k @ q[i, hd].double() / 8
+            best, second = x.topk(2).values.tolist() if len(x) > 1 else (x[0].item(), -math.inf)
+            # float32's sums of 64 products: 16 additions of a chain, and two
+            # products, of sums of |q k| / 8, on both sides; 40 beyond leaves e^-40.
+            terms = (k.abs() @ q[i, hd].double().abs()).max().item() / 8
+            if best - second > 2 * 20 * 2.0 ** -24 * terms + 40:
+                sure += 1
+                far = (out[i, hd] - v[x.argmax()]).abs()
+                assert bool((far <= half_step(dtype) * v[x.argmax()].abs() + 2.0 ** -25).all()), (i, hd)
+    assert sure > 0
+
+
+@pytest.mark.parametrize("dtype,size", [(FH, 700), (FH, 6000), (FH, 12000), (BF, 12000), (BF, 1e9)])
+def test_chunks_of_far_scores(device, dtype, size):
+    check_far_scores(dtype, 64, 1500, 600, 32, size)
