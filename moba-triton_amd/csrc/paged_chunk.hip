@@ -42,6 +42,7 @@ template <> struct Unit<bf16_t> {
   typedef bf16x8_t vec;
   typedef __bf16 scalar;
   static constexpr uint32_t kInf = 0x7f80u;
+  static constexpr float kShift = 0.f;
   __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -50,6 +51,7 @@ template <> struct Unit<f16_t> {
   typedef f16x8_t vec;
   typedef _Float16 scalar;
   static constexpr uint32_t kInf = 0x7c00u;
+  static constexpr float kShift = 15.f;  // weights up to 2^15: the second parts of small ones stay in range
   __device__ static floatx16_t mma(vec a, vec b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -240,8 +242,10 @@ __device__ inline int swizzle_v(int row) {
 //   S^T[key][entry] = K . Q^T,   O^T[feature][entry] = V^T . P^T
 // by 32x32x16 MFMAs; P^T goes from the first product's registers to the
 // second's operand (its keys in the order 8 (u / 4) + 4 h + u % 4 of lane half
-// h, which the values' reads follow). P is rounded to the type for the
-// product, as the framework's forward does; m, l and the partial rows stay in
+// h, which the values' reads follow). P goes as two numbers of the type, the
+// rounded weight and what the rounding left: 16 bits of it in bf16, 22 in fp16,
+// where one number's 8 and 11 would add as much error as the rounding of the
+// result does (0.0021 against 0.0017 in bf16). m, l and the partial rows stay in
 // float32. (Rows as 16-bit codes with a unit per 64 features move half the bytes
 // and coarsen the features beside a large one: values with one channel of 64
 // 1000 times the others' came out 0.9% off.)
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
     }
     const bool whole = __all(!live || lim == KEYS - 1);
     float m = -INFINITY, l = 0.f;
-    V8 bp[KEYS / 16];
+    V8 bp[KEYS / 16], bl[KEYS / 16];
     if (work) {
       // s[kt][v] is key 32 kt + 8 (v / 4) + 4 h + v % 4.
       if (!whole) {
@@ -410,13 +414,13 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
         for (int v = 0; v < 16; ++v) m = fmaxf(m, s[kt][v]);
       m = fmaxf(m, __shfl_xor(m, 32));
       const float mz = m > -INFINITY ? m : 0.f;
-      m *= a.scale_log2;
+      m = m * a.scale_log2 - M::kShift;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          // The difference first: at most 1 however large the scores are.
-          const float p = __builtin_amdgcn_exp2f((s[kt][v] - mz) * a.scale_log2);
+          // The difference first: at most 2^kShift however large the scores are.
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[kt][v] - mz, a.scale_log2, M::kShift));
           s[kt][v] = p;
           l += p;
         }
@@ -424,8 +428,11 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
 #pragma unroll
       for (int j = 0; j < KEYS / 16; ++j)
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          bp[j][u] = static_cast<typename M::scalar>(s[j >> 1][8 * (j & 1) + u]);
+        for (int u = 0; u < 8; ++u) {
+          const float p = s[j >> 1][8 * (j & 1) + u];
+          bp[j][u] = static_cast<typename M::scalar>(p);
+          bl[j][u] = static_cast<typename M::scalar>(p - static_cast<float>(bp[j][u]));
+        }
     }
     if (more)
       wait_loads<LOADS>();  // all but the next keys
@@ -459,23 +466,44 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
         meet();
       }
     }
-    // Two feature tiles at a time, kept until the queries are in.
-    floatx16_t o[DT];
+    // Two feature tiles at a time.
     if (work) {
+      if (live && h == 0) a.part_ml[ent] = make_float2(m, l);
       auto half = [&](auto pc) {
         constexpr int dt = 2 * decltype(pc)::value;
-        o[dt] = o[dt + 1] = floatx16_t{};
+        floatx16_t o[2] = {floatx16_t{}, floatx16_t{}};
         // Features 32 dt + [0, 64), keys 16 j + [0, 16).
         auto step = [&](auto jc) {
           constexpr int j = decltype(jc)::value;
           u32x2 x[4];
           read_transposed<64 * dt, j * 16 * D * 2>(v_at, v_at8, x);
-          o[dt] = M::mma(__builtin_bit_cast(V8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]}), bp[j], o[dt]);
-          o[dt + 1] = M::mma(__builtin_bit_cast(V8, u32x4{x[2][0], x[2][1], x[3][0], x[3][1]}), bp[j], o[dt + 1]);
+          const V8 y[2] = {__builtin_bit_cast(V8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]}),
+                           __builtin_bit_cast(V8, u32x4{x[2][0], x[2][1], x[3][0], x[3][1]})};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) o[t] = M::mma(y[t], bp[j], o[t]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) o[t] = M::mma(y[t], bl[j], o[t]);
         };
         steps(std::make_integer_sequence<int, KEYS / 16>{}, step);
-        if (bad) {
-          // What the queries see of the values that were taken out.
+        // The second parts of weights, zeros and negative numbers among them,
+        // make NaN of an infinite value.
+        uint32_t lost = 0;
+        if (!d.masked) {
+          float z = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) z = fmaf(o[e / 16][e % 16], 0.f, z);
+          if (__any(z != z)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = o[e / 16][e % 16];
+              lost |= x != x ? 1u << e : 0u;
+              o[e / 16][e % 16] = x != x ? 0.f : x;
+            }
+          }
+        }
+        const bool again = __any(lost);
+        if (bad || again) {
+          // What the queries see of the values that were taken out or lost.
           for (int key = 0; key < d.key_lim; ++key) {
             const uint16_t* row = d.v + key * D + 32 * dt + 4 * h;
 #pragma unroll
@@ -487,25 +515,31 @@ __global__ void __launch_bounds__(256, (kResident<D, KT>)) attend_columns_kernel
                 for (int w = 0; w < 4; ++w) {
                   const uint16_t bits = static_cast<uint16_t>(x[w >> 1] >> (16 * (w & 1)));
                   if ((bits & M::kInf) == M::kInf && key <= lim)
-                    o[dt + t][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
+                    o[t][4 * q4 + w] += static_cast<float>(__builtin_bit_cast(typename M::scalar, bits));
                 }
               }
           }
+        }
+        if (again) {  // sums of finite values that left the range
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = o[e / 16][e % 16];
+            o[e / 16][e % 16] = (lost >> e) & 1u && x == 0.f ? NAN : x;
+          }
+        }
+        if (live) {
+          float* dst = a.part_acc + static_cast<int64_t>(ent) * D + 32 * dt + 4 * h;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              *reinterpret_cast<float4*>(dst + t * 32 + 8 * q4) =
+                  make_float4(o[t][4 * q4], o[t][4 * q4 + 1], o[t][4 * q4 + 2], o[t][4 * q4 + 3]);
         }
       };
       steps(std::make_integer_sequence<int, DT / 2>{}, half);
     }
     have_query();
-    if (live && work) {
-      if (h == 0) a.part_ml[ent] = make_float2(m, l);
-      float* dst = a.part_acc + static_cast<int64_t>(ent) * D + 4 * h;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<float4*>(dst + dt * 32 + 8 * q4) =
-              make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
-    }
     meet();  // every wave is done with the values
     if (!more) break;
     load_values(next);

@@ -229,6 +229,47 @@ def test_the_largest_values_in_a_chunk(device):
     check_largest_values(64, 1500, 600, 32)
 
 
+def check_weights(dtype, block, length, n, h):
+    """Weights are no rounder than float32 sums show: scores without rounding
+    (one feature of a query counts), three keys of a block that matter, at s = 0
+    and close below, and others whose weights are exactly 0.
+
+    Roundings of float32, relative to the weighted mean of |v|: the scale and
+    the two numbers that the exponent is formed of, at most 17 in size, 35 times
+    ln 2; exp2 2; at most 12 weights summed, and as two numbers each in the
+    product, 36; four blocks merged, 8: under 80, in the row and in its sum. A
+    weight in two numbers of the type is off by half a step squared."""
+    d = 64
+    p = Paged([length], 1, block, d, dtype, 26)
+    real = p.k.isfinite()
+    p.k[real] = -24.0
+    for j, page in enumerate(p.table[0].tolist()):
+        for i, row in enumerate((1, block // 2, block - 2)):
+            p.k[page, 0, row] = torch.where(p.k[page, 0, row].isfinite(),
+                                            -torch.arange(d).add(j * 5 + i * 7).remainder(13) / 64, math.nan).to(dtype)
+    q = torch.zeros(n, h, d, dtype=dtype)
+    for i in range(n):
+        for hd in range(h):
+            q[i, hd, (i * 3 + hd * 11) % d] = 96.0
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    cache, table, lens = p.gpu()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg).cpu()
+    out = paged_attention(q.cuda(), cache, table, lens, cfg).cpu().double()
+    for i in range(0, n, max(1, n // 25)):
+        for hd in range(h):
+            ref, mean, _, _ = attend_exactly(p, q[i, hd], [j for j in ids[i, hd].tolist() if j >= 0], length - n + i)
+            bound = half_step(dtype) * ref.abs() + (half_step(dtype) ** 2 + 160 * 2.0 ** -24) * mean
+            if dtype == FH:
+                bound = bound + 2.0 ** -25
+            far = (out[i, hd] - ref).abs()
+            assert bool((far <= bound).all()), (i, hd, (far / bound).max().item())
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+def test_weights_of_a_chunk_keep_their_bits(device, dtype):
+    check_weights(dtype, 64, 1500, 600, 32)
+
+
 def check_far_scores(dtype, block, length, n, h, size):
     """Scores so large that neighbours are far apart in float32: nothing but the
     best key of every query counts, and no weight leaves the type's range."""
