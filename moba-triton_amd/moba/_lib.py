@@ -221,16 +221,24 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
 
 def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` itself where its rows (the last axis) can be read in 16-byte pieces
-    at its strides, else a contiguous copy."""
+    at its strides (`row_strides`), else a contiguous copy."""
     piece = 16 // t.element_size()
     *outer, last = t.stride()
     if last == 1 and t.data_ptr() % 16 == 0:
-        for s in outer:
-            if s % piece:
+        for n, s in zip(t.shape, outer):
+            if s % piece and n > 1:
                 break
         else:
             return t
     return aligned_contiguous(t)
+
+
+def row_strides(t: torch.Tensor) -> list[int]:
+    """Strides of all axes but the last of a tensor from `aligned_rows`. An
+    axis of size 1 may have any stride, which copies keep (torch calls the
+    tensor contiguous): 0 where it is none of 16-byte pieces."""
+    piece = 16 // t.element_size()
+    return [s if s % piece == 0 else 0 for s in t.stride()[:-1]]
 
 
 def aligned_contiguous(t: torch.Tensor) -> torch.Tensor:

@@ -188,7 +188,7 @@ def append_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Page
     if k_weight is not None:
         k_weight = k_weight.contiguous()
     call.q = q.data_ptr()
-    strides = _Strides(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    strides = _Strides(*_lib.row_strides(q), *_lib.row_strides(k), *_lib.row_strides(v))
     a = _lib.addr
     _lib.call_on(dev, "moba_append_tokens", ctypes.byref(call), k.data_ptr(), v.data_ptr(), strides,
                  out.data_ptr(), a(cos), a(sin), a(q_weight), a(k_weight), rotary, length,

@@ -99,7 +99,7 @@ _Strides = ctypes.c_int64 * 6
 
 
 def _shape_args(q, k, cos, code, eps, interleaved):
-    strides = _Strides(*q.stride()[:3], *k.stride()[:3])
+    strides = _Strides(*_lib.row_strides(q), *_lib.row_strides(k))
     rotary, length = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
     b, s, h, d = q.shape
     return (b, s, h, k.shape[2], d, strides, rotary, length, interleaved, eps,

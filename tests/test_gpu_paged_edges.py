@@ -33,6 +33,25 @@ def one_by_one(p, new, q, cfg):
     return torch.cat(ids), torch.cat(out), torch.cat(lse, 1)
 
 
+# -- layouts ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("h", [1, 4])
+def test_one_token_of_odd_rows(device, dtype, h):
+    """A token of a projection whose rows are no multiple of 16 bytes, appended:
+    the pages and queries of contiguous tensors."""
+    d, block = 64, 16
+    p = Paged([block], 1, block, d, dtype, 28)
+    x = p.randn(1, (h + 2) * d + 5).cuda()
+    q, k, v = x[:, :h * d].unflatten(1, (h, d)), x[:, None, h * d:h * d + d], x[:, None, h * d + d:h * d + 2 * d]
+    got = []
+    for q, k, v in ((q, k, v), [torch.empty(t.shape, dtype=dtype, device="cuda").copy_(t) for t in (q, k, v)]):
+        cache, table, lens = p.gpu()
+        got.append([append_tokens(q, k, v, cache, table, lens), cache.k, cache.v, cache.kbar])
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # -- scores that are not numbers --------------------------------------------------
 
 def check_scores_that_are_not_numbers(dtype, d, block, length, n, h, hk=2):
