@@ -22,6 +22,7 @@ struct RowArgs {
   float* lse;                // [h_q, tokens] log2 units, or null
   float* part_ml;            // [rows, splits, 2]
   float* part_o;             // [rows, splits, D]
+  int64_t row0;              // first row of this launch
   int h_q, h_kv, slots, splits;
   int take, current;
   float scale_log2;
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(64 * NW) attend_rows_kernel(RowArgs a) {
   __shared__ float s_m[NW], s_l[NW];
   __shared__ typename Best::Word s_best[NW][TS];
   __shared__ int32_t s_ids[TS + 1];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
   const int32_t tok = static_cast<int32_t>(row / a.h_q);
   const int h = static_cast<int>(row % a.h_q);
   const int hk = h / (a.h_q / a.h_kv);
@@ -389,11 +390,17 @@ static int run_attend(const moba_paged* c, const uint32_t* keys, void* stream) {
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
     auto go = [&](auto dim, auto nw, auto tm) {
       constexpr int D = decltype(dim)::value, NW = decltype(nw)::value, TM = decltype(tm)::value;
-      hipLaunchKernelGGL((attend_rows_kernel<T, D, NW, TM>),
-                         dim3(static_cast<unsigned>(rows), static_cast<unsigned>(a.splits)),
-                         dim3(64 * NW), 0, s, a);
-      int rc = check_launch("moba_paged_attend");
-      if (rc || a.splits == 1) return rc;
+      // A launch holds fewer than 2^32 threads (per axis).
+      constexpr int64_t most = (int64_t(1) << 32) / (64 * NW) - 1;
+      int rc = MOBA_OK;
+      for (a.row0 = 0; a.row0 < rows && !rc; a.row0 += most) {
+        const int64_t n = rows - a.row0 < most ? rows - a.row0 : most;
+        hipLaunchKernelGGL((attend_rows_kernel<T, D, NW, TM>),
+                           dim3(static_cast<unsigned>(n), static_cast<unsigned>(a.splits)),
+                           dim3(64 * NW), 0, s, a);
+        rc = check_launch("moba_paged_attend");
+      }
+      if (rc || a.splits == 1) return rc;  // splits: of at most a few thousand rows
       hipLaunchKernelGGL((merge_rows_kernel<T, D>), dim3(static_cast<unsigned>(rows)), dim3(64), 0, s, a);
       return check_launch("moba_paged_attend (merge)");
     };

@@ -596,8 +596,9 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
 
 // Rows of no sequence: all -1. One wave per token.
 __global__ void __launch_bounds__(64) nobody_kernel(GateArgs a) {
-  if (locate(a.p, blockIdx.x).pos >= 0) return;
-  int32_t* out = a.block_idx + static_cast<int64_t>(blockIdx.x) * a.h_q * a.slots;
+  const int32_t tok = a.tok0 + static_cast<int32_t>(blockIdx.x);
+  if (locate(a.p, tok).pos >= 0) return;
+  int32_t* out = a.block_idx + static_cast<int64_t>(tok) * a.h_q * a.slots;
   for (int i = threadIdx.x; i < a.h_q * a.slots; i += 64) out[i] = -1;
 }
 
@@ -608,13 +609,16 @@ __global__ void __launch_bounds__(64) nobody_kernel(GateArgs a) {
 // one of 512 blocks, 64 tokens (2048 rows) 46 and 32. 8 heads of 64, 8
 // sequences of 64 blocks, 64 tokens each (4096 rows) 21 and 31, 8 each 21 and 16.
 constexpr int64_t kTileRows = 4096;
+constexpr int64_t kMaxBlocks = int64_t(1) << 24;  // workgroups of 256 threads: a launch holds fewer than 2^32
 bool tiles_take(const moba_paged& c) {
   return c.dtype != MOBA_FP32 && c.take > 0 && c.table_width < (1 << 15) && c.h_q / c.h_kv <= 128 &&
-         c.h_kv <= 65535 && c.tokens >= 4 * c.seqs && c.tokens * c.h_q >= kTileRows;
+         c.h_kv <= 65535 && c.tokens >= 4 * c.seqs && c.tokens * c.h_q >= kTileRows &&
+         c.seqs * c.h_kv < kMaxBlocks && c.tokens / (128 / (c.h_q / c.h_kv)) + c.seqs < kMaxBlocks;
 }
 
 int64_t score_slice(const moba_paged& c) {
-  const int64_t n = (int64_t(1) << 24) / (c.h_q * c.table_width);
+  int64_t n = (int64_t(1) << 24) / (c.h_q * c.table_width);
+  if (n * c.h_kv >= kMaxBlocks) n = kMaxBlocks / 2 / c.h_kv;
   return n < 1 ? 1 : (n < c.tokens ? n : c.tokens);
 }
 
@@ -639,8 +643,11 @@ int run_tiles(const moba_paged& c, GateArgs a, bool all_rows, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
       hipLaunchKernelGGL((norm_kernel<T, D / 16>), dim3(static_cast<unsigned>(c.seqs * c.h_kv), kNormParts),
                          dim3(256), 0, s, a);
-      if (all_rows)
-        hipLaunchKernelGGL(nobody_kernel, dim3(static_cast<unsigned>(c.tokens)), dim3(64), 0, s, a);
+      for (int64_t t0 = 0; all_rows && t0 < c.tokens; t0 += kMaxBlocks) {
+        a.tok0 = static_cast<int32_t>(t0);
+        const int64_t n = c.tokens - t0 < kMaxBlocks ? c.tokens - t0 : kMaxBlocks;
+        hipLaunchKernelGGL(nobody_kernel, dim3(static_cast<unsigned>(n)), dim3(64), 0, s, a);
+      }
       auto go = [&](auto m, auto tm) {
         hipLaunchKernelGGL((tiles_kernel<T, D, decltype(m)::value, decltype(tm)::value>),
                            dim3(static_cast<unsigned>(parts), static_cast<unsigned>(c.h_kv)), dim3(256), 0, s, a);

@@ -298,6 +298,8 @@ extern "C" int moba_append_tokens(const moba_paged* c, const void* k_new, const 
   dim3 grid(static_cast<unsigned>(runs < a.p.tokens ? runs : a.p.tokens),
             static_cast<unsigned>(a.h_kv + cdiv(a.h_q, kQHeads)));
   if (grid.y > 65535) return fail(MOBA_ERR_UNSUPPORTED, "append: too many heads");
+  if (grid.x >= 1u << 24)  // of 256 threads: a launch holds fewer than 2^32
+    return fail(MOBA_ERR_UNSUPPORTED, "append: too many tokens");
   return MOBA_DISPATCH_DTYPE(static_cast<int>(c->dtype), T, [&] {
     auto run = [&](auto lpr, auto il) {
       hipLaunchKernelGGL((append_kernel<T, decltype(lpr)::value, decltype(il)::value>), grid, dim3(kAppendThreads), 0,

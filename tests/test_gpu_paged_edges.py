@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from moba.config import MoBAConfig
-from moba.kernels.paged import append_tokens, paged_attention, paged_gate_select
+from moba.kernels.paged import PagedKV, append_tokens, paged_attention, paged_gate_select
 from paged_util import Paged, cu_of, half_step
 
 pytestmark = pytest.mark.gpu
@@ -327,3 +327,25 @@ def check_far_scores(dtype, block, length, n, h, size):
 @pytest.mark.parametrize("dtype,size", [(FH, 700), (FH, 6000), (FH, 12000), (BF, 12000), (BF, 1e9)])
 def test_chunks_of_far_scores(device, dtype, size):
     check_far_scores(dtype, 64, 1500, 600, 32, size)
+
+
+# -- sizes ------------------------------------------------------------------------
+
+def test_more_rows_than_a_launch_holds(device):
+    """2^24 query rows and more, each with its own block only: the last sequence
+    has the result that it has by itself."""
+    seqs, n, h, d, block = 8, 65541, 32, 64, 16
+    assert seqs * n * h > 1 << 24
+    cfg = MoBAConfig(block_size=block, top_k=1, dtype=F32)
+    width = -(-n // block)
+    g = torch.Generator(device="cuda").manual_seed(29)
+    q = torch.randn(seqs * n, h, d, generator=g, device="cuda")
+    k, v = (torch.randn(seqs * width, 1, block, d, generator=g, device="cuda") for _ in range(2))
+    cache = PagedKV(k, v, torch.zeros(seqs * width, 1, d, device="cuda"))
+    table = torch.arange(seqs * width, dtype=torch.int32, device="cuda").view(seqs, width)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    out, lse = paged_attention(q, cache, table, lens, cfg, return_lse=True)
+    for s in (0, seqs - 1):
+        at = slice(s * n, s * n + n)
+        want, want_lse = paged_attention(q[at], cache, table[s:s + 1], lens[:1], cfg, return_lse=True)
+        assert torch.equal(out[at], want) and torch.equal(lse[:, at], want_lse)
