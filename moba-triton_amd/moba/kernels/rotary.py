@@ -12,6 +12,7 @@ No counterpart in the reference, whose inputs come normed and rotated.
 import ctypes
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from moba import _lib
@@ -155,7 +156,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
     """Queries and keys normed per head and rotated by position, with gradient
     support for q, k and the weights. Computed in float32, rounded once. In a
     captured graph take the gradients with `torch.autograd.grad`, of leaves that
-    no live eager graph shares.
+    no live eager graph shares. Forward-mode derivatives are refused.
 
     Args:
         q: [B, S, H_q, D]; k: [B, S, H_kv, D]. Any strides (views of one fused
@@ -174,6 +175,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
 
     Raises:
         ValueError: On mismatched shapes, dtypes, tables or weights.
+        RuntimeError: On dual tensors (forward-mode).
     """
     code, rotary = _check(q, k, cos, sin, positions, q_weight, k_weight)
     _lib.require_gpu(q, k, q_weight, k_weight, cos, sin, positions)
@@ -190,9 +192,9 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
             positions = positions.clamp(-1, 2 ** 31 - 1)
         positions = positions.to(torch.int32).expand(q.shape[:2]).contiguous()
     args = (q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), code)
-    if torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or
-            (q_weight is not None and q_weight.requires_grad) or
-            (k_weight is not None and k_weight.requires_grad)):
-        return NormRotateFunction.apply(*args)
+    grad = torch.is_grad_enabled()
+    for t in (q, k, q_weight, k_weight):
+        # Tangents of forward-mode go there too, to be refused.
+        if t is not None and (grad and t.requires_grad or unpack_dual(t).tangent is not None):
+            return NormRotateFunction.apply(*args)
     return _forward(*args)

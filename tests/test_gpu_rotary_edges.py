@@ -1,7 +1,9 @@
-"""norm_rotate at the edges of what it takes: one token, one head."""
+"""norm_rotate at the edges of what it takes: one token, one head,
+forward-mode derivatives."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from moba.kernels.rotary import norm_rotate
 from paged_util import tables
@@ -33,3 +35,20 @@ def test_one_token_or_head_of_odd_rows(device, dtype, batch, seq, h, hk):
                torch.empty(k.shape, dtype=dtype, device="cuda").copy_(k))
     for a, b in zip(run(q, k), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "q_weight", "k_weight"])
+def test_forward_mode_is_refused(device, which):
+    """A tangent is never dropped in silence, with gradients enabled or not."""
+    args = {"q": torch.randn(1, 3, 2, 64, device="cuda"), "k": torch.randn(1, 3, 1, 64, device="cuda"),
+            "q_weight": torch.rand(64, device="cuda"), "k_weight": torch.rand(64, device="cuda")}
+    cos, sin = (t.cuda() for t in tables(3, 64))
+    want = norm_rotate(**args, cos=cos, sin=sin)
+    with forward_ad.dual_level():
+        # Without a dual tensor the call stands.
+        for a, b in zip(norm_rotate(**args, cos=cos, sin=sin), want):
+            assert torch.equal(a, b)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward"):
+                norm_rotate(**args, cos=cos, sin=sin)
