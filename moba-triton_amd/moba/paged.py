@@ -12,7 +12,9 @@ work on the pages themselves is `moba.kernels.paged`'s. One decoding step:
                             cu_seqlens=step.cu_seqlens)
 """
 
+import ctypes
 import heapq
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -41,7 +43,7 @@ class Step:
 
 class _Sequence:
     def __init__(self, pages=(), length=0):
-        self.pages, self.length = list(pages), length
+        self.pages, self.length = array("i", pages), length
 
 
 class PagedCache:
@@ -101,12 +103,15 @@ class PagedCache:
     def grow(self, seqs: list[int], new: list[int]) -> Step:
         """Room for `new[i]` more tokens of sequence `seqs[i]`. A partly filled
         last page that others hold too is copied first (one `copy_pages` call
-        for all sequences).
+        for all sequences). Does not wait for the device.
 
         Raises:
             CacheFull: With too few free pages; nothing has changed then.
+            RuntimeError: While a graph is captured: the books would change
+                once, the step's tables with every replay.
             ValueError: If a sequence is named twice or a count is negative.
         """
+        self._outside_capture()
         if len(seqs) != len(new) or not seqs:
             raise ValueError(f"{len(seqs)} sequences, {len(new)} counts of new tokens")
         if len(set(seqs)) != len(seqs):
@@ -138,13 +143,14 @@ class PagedCache:
         if src:
             copy_pages(self.kv, src, dst)
         for s, n, g in zip(held, new, grown):
-            s.pages += [self._take() for _ in range(g)]
+            s.pages.extend(self._take() for _ in range(g))
             s.length += n
         return self._step(held, new)
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the cache; returns how many
-        moved. Block tables from before are stale."""
+        moved. Block tables from before are stale. Not in a captured graph."""
+        self._outside_capture()
         live = [p for p, n in enumerate(self._holders) if n]
         holes = [p for p in range(len(live)) if not self._holders[p]]
         move = dict(zip((p for p in live if p >= len(live)), holes))
@@ -152,11 +158,16 @@ class PagedCache:
             return 0
         copy_pages(self.kv, list(move), list(move.values()))
         for s in self._sequences.values():
-            s.pages = [move.get(p, p) for p in s.pages]
+            s.pages = array("i", (move.get(p, p) for p in s.pages))
         for a, b in move.items():
             self._holders[a], self._holders[b] = 0, self._holders[a]
         self._free = list(range(len(live), len(self._holders)))
         return len(move)
+
+    def _outside_capture(self) -> None:
+        if self.kv.k.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the books of a cache do not change in a captured graph: grow and "
+                               "compact outside of it, and capture the calls on their tables")
 
     def _of(self, seq: int) -> _Sequence:
         if seq not in self._sequences:
@@ -174,13 +185,19 @@ class PagedCache:
             heapq.heappush(self._free, page)
 
     def _step(self, held, new) -> Step:
-        width = max(1, max(len(s.pages) for s in held))
-        table = [s.pages + [-1] * (width - len(s.pages)) for s in held]
-        cu = [0]
+        width, lens = max(1, max(len(s.pages) for s in held)), len(held)
+        rows = lens * width
+        tail = array("i", (s.length for s in held))
+        tail.append(0)
         for n in new:
-            cu.append(cu[-1] + n)
-        # One copy to the device for all three.
-        flat = torch.tensor([*sum(table, []), *(s.length for s in held), *cu], dtype=torch.int32)
-        flat = flat.to(self.kv.k.device)
-        rows, lens = len(held) * width, len(held)
-        return Step(flat[:rows].view(len(held), width), flat[rows:rows + lens], flat[rows + lens:])
+            tail.append(tail[-1] + n)
+        # One copy to the device for all three, from pinned memory of its own:
+        # the host goes on, and the allocator keeps the memory until the copy
+        # is done.
+        device = self.kv.k.device
+        flat = torch.full((rows + 2 * lens + 1,), -1, dtype=torch.int32, pin_memory=device.type == "cuda")
+        for at, part in [(i * width, s.pages) for i, s in enumerate(held)] + [(rows, tail)]:
+            address, count = part.buffer_info()
+            ctypes.memmove(flat.data_ptr() + 4 * at, address, 4 * count)
+        flat = flat.to(device, non_blocking=True)
+        return Step(flat[:rows].view(lens, width), flat[rows:rows + lens], flat[rows + lens:])
