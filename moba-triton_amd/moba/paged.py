@@ -103,7 +103,8 @@ class PagedCache:
     def grow(self, seqs: list[int], new: list[int]) -> Step:
         """Room for `new[i]` more tokens of sequence `seqs[i]`. A partly filled
         last page that others hold too is copied first (one `copy_pages` call
-        for all sequences). Does not wait for the device.
+        for all sequences; where that fails, nothing has changed). Does not
+        wait for the device.
 
         Raises:
             CacheFull: With too few free pages; nothing has changed then.
@@ -134,14 +135,17 @@ class PagedCache:
         grown = [-(-(s.length + n) // bs) - len(s.pages) for s, n in zip(held, new)]
         if len(copies) + sum(grown) > len(self._free):
             raise CacheFull(f"{len(copies) + sum(grown)} pages needed, {len(self._free)} free")
-        src, dst = [], []
-        for s in copies:
-            src.append(s.pages[-1])
-            dst.append(self._take())
-            self._drop(s.pages[-1])
-            s.pages[-1] = dst[-1]
+        src, dst = [s.pages[-1] for s in copies], [self._take() for _ in copies]
         if src:
-            copy_pages(self.kv, src, dst)
+            try:
+                copy_pages(self.kv, src, dst)
+            except Exception:
+                for p in dst:
+                    self._drop(p)
+                raise
+        for s, p in zip(copies, dst):
+            self._drop(s.pages[-1])
+            s.pages[-1] = p
         for s, n, g in zip(held, new, grown):
             s.pages.extend(self._take() for _ in range(g))
             s.length += n

@@ -4,6 +4,8 @@ import pytest
 import torch
 
 from moba import _lib
+from moba import paged as P
+from moba.config import MoBAConfig
 
 BF = torch.bfloat16
 
@@ -28,3 +30,18 @@ def test_strides_of_axes_of_size_one(dtype, piece):
         strides = _lib.row_strides(rows)
         assert all(s % piece == 0 for s in strides)
         assert torch.equal(torch.as_strided(rows, t.shape, [*strides, 1], rows.storage_offset()), t)
+
+
+def test_a_failed_copy_changes_no_books():
+    """Page copies need a GPU: `grow` of a forked sequence fails here, and the
+    books stay as they were."""
+    c = P.PagedCache(2, 12, 2, 64, MoBAConfig(block_size=16, top_k=3), device="cpu")
+    a = c.create()
+    c.grow([a], [20])
+    b = c.fork(a)
+    before = (c.pages(a), c.pages(b), c.length(a), c.length(b), list(c._holders), sorted(c._free))
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        c.grow([a, b], [1, 40])
+    assert before == (c.pages(a), c.pages(b), c.length(a), c.length(b), list(c._holders), sorted(c._free))
+    c.free(b)
+    assert c.grow([a], [1]).block_table.tolist() == [[0, 1]]
