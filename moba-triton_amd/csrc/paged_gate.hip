@@ -328,14 +328,16 @@ __global__ void __launch_bounds__(256, 2) tiles_kernel(GateArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) qn = fmaf(static_cast<float>(bq[k][e]), static_cast<float>(bq[k][e]), qn);
   }
-  qn = sqrtf(qn + __shfl_xor(qn, 32)) * 1.0001f;
+  // Norms carry 2e-18 on top: up to 256 squares of less than 2^-126 each
+  // may be missing from their sums.
+  qn = sqrtf(qn + __shfl_xor(qn, 32)) * 1.0001f + 2e-18f;
   float kn = 0.f;
   {
     uint32_t best = 0;
     const uint32_t* norms = a.norms + (static_cast<int64_t>(pt.seq) * a.h_kv + hk) * kNormParts;
 #pragma unroll
     for (int i = 0; i < kNormParts; ++i) best = max(best, norms[i]);
-    kn = u2f(best) * 1.0001f;
+    kn = u2f(best) * 1.0001f + 2e-18f;
   }
   // Widened by the rounding of a -+ E itself, with |a| * 2.4e-7 below.
   const float E = (qn * kn * (D * 0x1p-23f) + (D + 1) * 1.2e-38f) * 1.001f;

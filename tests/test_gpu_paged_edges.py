@@ -8,7 +8,7 @@ import torch
 
 from moba.config import MoBAConfig
 from moba.kernels.paged import PagedKV, append_tokens, paged_attention, paged_gate_select
-from paged_util import Paged, cu_of, half_step
+from paged_util import Paged, cu_of, half_step, select64
 
 pytestmark = pytest.mark.gpu
 
@@ -31,6 +31,35 @@ def one_by_one(p, new, q, cfg):
             lse.append(e)
         at += n
     return torch.cat(ids), torch.cat(out), torch.cat(lse, 1)
+
+
+# -- representatives far below 1 --------------------------------------------------
+
+def check_small_representatives(length, n, h, unit):
+    """Representatives whose squares are below float32's smallest number, and
+    whose scores are what sums of their products lose: c + a - c, with a 2^-26
+    of c and another one for every block."""
+    d, block = 64, 16
+    p = Paged([length], 1, block, d, BF, 31)
+    blocks = torch.arange(length // block)
+    kbar = torch.zeros(len(blocks), 1, d)
+    kbar[:, 0, 0], kbar[:, 0, 32] = unit, -unit
+    kbar[:, 0, 16] = unit * 2.0 ** -26 * (1 + (blocks * 37 % 128) / 128)
+    p.kbar[p.table[0, :len(blocks)].long()] = kbar.to(BF)
+    q = torch.zeros(n, h, d, dtype=BF)
+    q[..., ::16] = 1.0
+    q[..., 48] = p.randn(n, h)
+    cfg = MoBAConfig(block_size=block, top_k=4)
+    cache, table, lens = p.gpu()
+    ids = paged_gate_select(q.cuda(), cache, table, lens, cfg).cpu()
+    for i in range(0, n, max(1, n // 10)):
+        want = select64(p, 0, q[i], length - n + i, cfg)
+        assert [x.tolist() for x in ids[i]] == want, i
+
+
+@pytest.mark.parametrize("unit", [2.0 ** -60, 2.0 ** -80, 2.0 ** -95])
+def test_small_representatives_of_a_chunk(device, unit):
+    check_small_representatives(2000, 300, 32, unit)
 
 
 # -- layouts ----------------------------------------------------------------------
