@@ -13,6 +13,7 @@ kernels, which treat what makes no sense as absent (see `append_tokens`).
 
 import ctypes
 from dataclasses import dataclass
+from operator import index
 
 import torch
 
@@ -294,7 +295,12 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor,
 
 
 def _page_list(pages, name):
-    t = pages if isinstance(pages, torch.Tensor) else torch.tensor(list(pages), dtype=torch.int32)
+    t = pages
+    if not isinstance(t, torch.Tensor):
+        try:
+            t = torch.tensor([index(p) for p in pages], dtype=torch.int32)
+        except (TypeError, RuntimeError) as exc:  # no whole numbers, or past 32 bits
+            raise ValueError(f"{name} must be a list of pages: {exc}") from None
     if t.ndim != 1 or t.dtype != torch.int32:
         raise ValueError(f"{name} must be a list of pages (int32, one axis)")
     return t.contiguous()

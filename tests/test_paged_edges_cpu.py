@@ -6,6 +6,7 @@ import torch
 from moba import _lib
 from moba import paged as P
 from moba.config import MoBAConfig
+from moba.kernels.paged import PagedKV, copy_pages
 
 BF = torch.bfloat16
 
@@ -45,3 +46,10 @@ def test_a_failed_copy_changes_no_books():
     assert before == (c.pages(a), c.pages(b), c.length(a), c.length(b), list(c._holders), sorted(c._free))
     c.free(b)
     assert c.grow([a], [1]).block_table.tolist() == [[0, 1]]
+
+
+@pytest.mark.parametrize("src,dst", [([0.7], [1]), ([0], [1.9]), ([0], ["1"]), ([0], [None]),
+                                     ([2 ** 31], [1]), ([0], [-2 ** 40]), ([[0]], [[1]])])
+def test_page_lists_of_no_pages(src, dst):
+    with pytest.raises(ValueError, match="must be a list of pages"):
+        copy_pages(PagedKV.empty(4, 1, 16, 64, BF, "cpu"), src, dst)
