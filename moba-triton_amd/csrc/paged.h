@@ -46,11 +46,22 @@ __device__ inline NewTokens new_tokens(const Paged& p, int32_t s) {
 // that no token has two sequences and their tokens are at most p.tokens in all.
 // `reach`: where the earlier ones end, 0 at first.
 __device__ inline NewTokens counted_tokens(const Paged& p, int32_t base, int32_t& reach) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, s = base + lane;
+  const bool in = s < p.seqs;
   NewTokens r{0, 0, 0};
-  if (base + lane < p.seqs) r = new_tokens(p, base + lane);
-  if (!p.cu) return r;
-  int32_t end = r.n ? r.first + r.n : 0;
+  if (!p.cu) return in ? new_tokens(p, s) : r;
+  int32_t first = 0, bound = 0;
+  if (in) {
+    first = p.cu[s];
+    bound = p.cu[s + 1];
+    r = checked_tokens(p, first, bound, p.seq_lens[s]);
+  }
+  int32_t end = r.n ? bound : 0;
+  if (!__ballot(bound < first || (r.n && first < reach))) {  // bounds that do not fall
+    const uint64_t some = __ballot(r.n > 0);
+    if (some) reach = __shfl(end, 63 - __builtin_clzll(some));
+    return r;
+  }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int32_t y = __shfl_up(end, off);
@@ -75,32 +86,41 @@ __device__ inline TokenAt token_at(int32_t s, const NewTokens& r, int32_t tok) {
   return TokenAt{s, i >= 0 && i < r.n ? r.len - r.n + i : -1};
 }
 
+// By counted_tokens' rule, whatever the bounds are.
+__device__ inline TokenAt locate_by_rule(const Paged& p, int32_t tok) {
+  int32_t reach = 0;
+  for (int32_t base = 0; base < p.seqs; base += 64) {
+    const NewTokens r = counted_tokens(p, base, reach);
+    const uint64_t holds = __ballot(r.n && r.first <= tok && tok < r.first + r.n);
+    if (!holds) continue;
+    const int l = __builtin_ctzll(holds);
+    return token_at(base + l, NewTokens{__shfl(r.first, l), __shfl(r.n, l), __shfl(r.len, l)}, tok);
+  }
+  return TokenAt{0, -1};
+}
+
 __device__ inline TokenAt locate(const Paged& p, int32_t tok) {
   if (!p.cu) {
     const int32_t s = tok / p.even;
     return token_at(s, new_tokens(p, s), tok);
   }
   const int lane = threadIdx.x & 63;
-  int32_t reach = 0;
+  int32_t most = INT32_MIN;  // the lane's largest bound so far
   for (int32_t base = 0; base < p.seqs; base += 64) {
-    NewTokens r = new_tokens(p, min(base + lane, p.seqs - 1));
-    if (base + lane >= p.seqs) r.n = 0;
-    const int32_t end = r.n ? r.first + r.n : 0;
-    const uint64_t holds = __ballot(r.first <= tok && tok < end);
-    if (holds) {
-      // As counted_tokens: the first one that holds the token or none, for it
-      // reaches behind the first tokens of the others that do.
-      const int l = __builtin_ctzll(holds);
-      const int32_t first = __shfl(r.first, l);
-      if (first < reach || __ballot(lane < l && end > first)) break;
-      return token_at(base + l, NewTokens{first, __shfl(r.n, l), __shfl(r.len, l)}, tok);
+    const int32_t i = min(base + lane, p.seqs - 1), end = p.cu[i + 1];
+    // Sequences up to the one that holds the token end at or before it.
+    const uint64_t behind = __ballot(base + lane < p.seqs && end > tok);
+    if (!behind) {
+      most = max(most, end);
+      continue;
     }
-    if (base + 64 < p.seqs) {
-      int32_t most = end;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off));
-      reach = max(reach, most);
-    }
+    const int l = __builtin_ctzll(behind);
+    const int32_t first = __shfl(p.cu[i], l);
+    const TokenAt at =
+        token_at(base + l, checked_tokens(p, first, __shfl(end, l), __shfl(p.seq_lens[i], l)), tok);
+    // It holds the token, and none before it reaches behind its first one.
+    if (at.pos >= 0 && !__ballot(most > first || (lane < l && end > first))) return at;
+    return locate_by_rule(p, tok);
   }
   return TokenAt{0, -1};
 }
