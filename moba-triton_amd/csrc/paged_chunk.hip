@@ -14,11 +14,11 @@
 //
 // 2048 tokens at the end of 129k, 32 and 8 heads of 128 in bf16, 8 blocks of 128
 // per query (0.5 million entries, 0.5 GB of keys and values that are each staged
-// once): 8 + 13 + 9 us of sorting, 177 of attention, 34 of merging. The
-// attention moves 0.67 GB, 3.8 TB/s: columns hold 64 entries on average, so half
+// once): 9 + 14 + 10 us of sorting, 208 of attention, 56 of merging. The
+// attention moves 0.8 GB, 3.8 TB/s: columns hold 64 entries on average, so half
 // of a workgroup's waves wait for the next block, and two workgroups share a CU's
-// LDS. 12 sequences with 1 to 700 tokens, 16 and 4 heads of 64 in fp16, 12 blocks
-// of 64: 23, 97 and 21 us.
+// LDS. The merge reads 0.27 GB of partial rows, 5.2 TB/s. 12 sequences with 1 to
+// 700 tokens, 16 and 4 heads of 64 in fp16, 12 blocks of 64: 24, 104 and 32 us.
 //
 // An entry is its index in block_idx, which is also the index of its partial
 // row. Entries of a column stand in no particular order; nothing depends on it.
@@ -250,8 +250,9 @@ __device__ inline int swizzle_v(int row) {
 // and coarsen the features beside a large one: values with one channel of 64
 // 1000 times the others' came out 0.9% off.)
 // kResident workgroups share a CU, as registers and LDS let them, and the grid
-// has as many: each has one item's loads under way (D 64, blocks of 64, the fp16
-// call above: three 97 us, two 106; four would spill).
+// has as many: each has one item's loads under way (D 64, blocks of 64, 12 sequences
+// of 350 new fp16 tokens, all of the attention: three 170 us, two 176; four would
+// spill).
 template <int D, int KT>
 constexpr int kResident = D * KT <= 64 ? 4 : D * KT <= 128 ? 3 : 2;
 
@@ -618,16 +619,17 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Block by block pays where an entry's block is on average another's too, and
 // where the entries' keys and values, which rows read one by one, outweigh the
-// launches. bf16, 32 and 8 heads of 128, 9 blocks of 128 per query, block by
-// block and row by row: 32 sequences of 256 blocks, 4 new tokens each (0.6
-// entries per block) 352 and 315 us, 8 each (1.1) 553 and 586, 16 each 772 and
-// 1130; one of 512 blocks, 8 tokens 48 and 27, 64 tokens (1.2 GB) 79 and 148. 8
-// heads of 64, 5 blocks of 64: 8 of 64 blocks, 64 tokens each (335 MB) 47 and 32.
+// launches. bf16, 32 and 8 heads of 128, 9 blocks of 128 per query, whole calls
+// block by block and row by row: 32 sequences of 256 blocks, 4 new tokens each
+// (0.6 entries per block) 413 and 314 us, 8 each (1.1) 631 and 577, 16 each (2.2)
+// 855 and 1102; one of 512 blocks, 8 tokens 65 and 27, 32 tokens (0.6 GB) 88 and
+// 77, 64 tokens (1.2 GB) 98 and 145. 8 heads of 64, 5 blocks of 64: 8 of 64 blocks,
+// 64 tokens each (335 MB) 43 and 32, 128 tokens each (671 MB) 49 and 58.
 constexpr int64_t kColumnBytes = int64_t(1) << 29;
 bool chunk_takes(const moba_paged& c) {
   const int64_t entries = c.tokens * c.h_q * c.slots;
   return c.dtype != MOBA_FP32 && (c.head_dim == 64 || c.head_dim == 128) && c.block_size <= 128 &&
-         c.table_width <= 15360 && c.h_kv <= 65535 && entries >= c.seqs * c.h_kv * c.table_width &&
+         c.table_width <= 15360 && c.h_kv <= 65535 && 2 * entries >= 3 * c.seqs * c.h_kv * c.table_width &&
          entries * c.block_size * c.head_dim * 4 >= kColumnBytes;
 }
 
@@ -638,8 +640,8 @@ ChunkPlan chunk_plan(const moba_paged& c) {
   pl.slice = (int64_t(1) << 29) / (per_token * c.head_dim * 4);
   pl.slice = pl.slice < 1 ? 1 : (pl.slice < c.tokens ? pl.slice : c.tokens);
   // Parts of 64 tokens: more workgroups count and place, and the scan walks more
-  // parts (4 x 512 tokens, 4 kv heads: the attention 157 us, in parts of 256
-  // 189; 2048 tokens, 8 kv heads: 255 and 256). Longer ones where a slice has
+  // parts (4 x 512 tokens, 4 kv heads: the attention 224 us, in parts of 256
+  // 255; 2048 tokens, 8 kv heads: 307 and 308). Longer ones where a slice has
   // more than 64 of them or the count table would pass 2^22 entries.
   pl.part = 64;
   while (pl.slice / pl.part > 64) pl.part *= 2;
