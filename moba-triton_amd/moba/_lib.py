@@ -225,10 +225,12 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     piece = 16 // t.element_size()
     *outer, last = t.stride()
     if last == 1 and t.data_ptr() % 16 == 0:
-        for n, s in zip(t.shape, outer):
-            if s % piece and n > 1:
+        for s in outer:
+            if s % piece:
                 break
         else:
+            return t
+        if all(n == 1 or s % piece == 0 for n, s in zip(t.shape, outer)):
             return t
     return aligned_contiguous(t)
 
