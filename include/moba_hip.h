@@ -328,7 +328,7 @@ int moba_backward_step(moba_step* step, void* stream);
  * head of q, then of k; elements, multiples of 16 bytes, features next to
  * each other); q_out, k_out contiguous. cos / sin [table_len, rotary / 2]
  * float32. positions [batch * seq] int32, or NULL: 0, 1, .. in every row; a
- * position outside the table gives NaN rows. Weights [D] of weight_dtype
+ * position outside the table gives NaN in the rotated features. Weights [D] of weight_dtype
  * (float32 or the input dtype), or NULL. head_dim a power of two from 32 to
  * 1024, rotary a multiple of 16. Rows on 16-byte boundaries.
  * The backward takes the outputs' gradients (contiguous) and writes dq, dk

@@ -163,12 +163,12 @@ __global__ void __launch_bounds__(256) select_kernel(GateArgs a) {
 // lists' last; the other queries (constructed ties, infinities, NaN) score
 // every block exactly.
 //
-// 2048 tokens of 32 and 8 heads of 128 over 1008 blocks, take 7, bf16: 87 us (the
+// 2048 tokens of 32 and 8 heads of 128 over 1008 blocks, take 7, bf16: 90 us (the
 // products of both passes take 28 at the rate of a large product; one pass that
 // keeps sorted lists as it goes took 168 for the lists alone). What is left is
 // VALU work at two waves per SIMD, which the grid has: the candidates and the
 // exact scores. 3396 tokens of 12 sequences, 16 and 4 heads of 64 in fp16, take
-// 11: 79 us.
+// 11: 81 us.
 constexpr int kNormParts = 16;
 
 template <typename T> struct GateUnit;

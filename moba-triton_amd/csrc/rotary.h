@@ -29,7 +29,8 @@ __device__ inline RotLane rot_lane(int lane, int rotary, int interleaved) {
 }
 
 // The lane's cosines and sines of position `pos`. A position outside the
-// table gives NaN, and so NaN rows: nothing outside the table is read.
+// table gives NaN, and so do the rotated features: nothing outside the table is
+// read.
 __device__ inline void rot_turn(const RotLane& r, const float* cosv, const float* sinv, int rotary,
                                 int64_t pos, int64_t table_len, float (&c)[8], float (&s)[8]) {
   const bool ok = pos >= 0 && pos < table_len;

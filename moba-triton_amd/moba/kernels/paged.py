@@ -253,7 +253,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor,
                     return_lse: bool = False):
     """MoBA attention of new tokens over a cache that already holds them
     (`append_tokens`): a chunk of each prompt, or the one token of a decoding
-    step. The result is `moba_attention`'s for the same tokens.
+    step. The result is `moba_attention`'s for the same tokens but for
+    roundings. A call's sizes decide how its tokens are computed: by float32
+    alone, or, in 16-bit chunks, with weights of 16 (bf16) or 22 (float16)
+    bits in the product and float32 sums; the same token in a chunk and by
+    itself may differ by a step of its type.
 
     Args:
         q: [T, H_q, D], normed and rotated.

@@ -164,7 +164,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None,
         cos, sin: float32 [positions, rotary / 2], rotary a multiple of 16 of
             at most D; None: no rotation.
         positions: int32 / int64 [B, S] or [S]; None: 0, 1, .. in each row. A
-            position outside the tables gives NaN rows.
+            position outside the tables gives NaN in the rotated features.
         q_weight, k_weight: [D], float32 or of q's dtype; None: that tensor is
             not normed.
         interleaved: Rotate neighbours (2i, 2i + 1) instead of halves
