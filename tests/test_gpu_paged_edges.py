@@ -378,3 +378,38 @@ def test_more_rows_than_a_launch_holds(device):
         at = slice(s * n, s * n + n)
         want, want_lse = paged_attention(q[at], cache, table[s:s + 1], lens[:1], cfg, return_lse=True)
         assert torch.equal(out[at], want) and torch.equal(lse[:, at], want_lse)
+
+
+@pytest.mark.parametrize("dtype,d,block", [(FH, 64, 64), (BF, 128, 128)])
+def test_chunks_of_several_slices(device, dtype, d, block):
+    """A call whose partial rows take more than one slice of scratch, prompts from
+    an empty cache and a chunk behind one, slices ending inside sequences: every
+    sequence has the bits that it has by itself."""
+    h, hk, ctx, new = 32, 2, [0, 100, 0], [9000, 700, 11000]
+    cfg = MoBAConfig(block_size=block, top_k=4, dtype=dtype)
+    assert sum(new) * h * 4 * d * 4 > 2 ** 29
+    g = torch.Generator(device="cuda").manual_seed(32)
+    lens = [c + n for c, n in zip(ctx, new)]
+    counts = [-(-n // block) for n in lens]
+    pages, width = sum(counts) + 1, max(counts)
+    k, v = (torch.randn(pages, hk, block, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    cache = PagedKV(k, v, k.float().mean(2).to(dtype))
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    for s, n in enumerate(counts):
+        table[s, :n] = order[sum(counts[:s]):sum(counts[:s]) + n]
+    q = torch.randn(sum(new) + 5, h, d, generator=g, device="cuda").to(dtype)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 5.0)
+    _, lse = paged_attention(q, cache, table, seq_lens, cfg, cu_seqlens=cu_of(new).cuda(), out=out, return_lse=True)
+    assert bool((out[sum(new):] == 5).all())
+    at = 0
+    for s, n in enumerate(new):
+        part = slice(at, at + n)
+        want, want_lse = paged_attention(q[part], cache, table[s:s + 1], seq_lens[s:s + 1], cfg, return_lse=True)
+        assert torch.equal(out[part], want) and torch.equal(lse[:, part], want_lse), s
+        # The last tokens again, in a call that has others in its slice.
+        tail, tail_lse = paged_attention(q[at + n - 400:at + n], cache, table[s:s + 1], seq_lens[s:s + 1], cfg,
+                                         return_lse=True)
+        assert torch.equal(out[at + n - 400:at + n], tail) and torch.equal(lse[:, at + n - 400:at + n], tail_lse), s
+        at += n
